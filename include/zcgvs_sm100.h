@@ -57,7 +57,8 @@ typedef enum zcgvs_dtype {
     ZCGVS_DTYPE_F16 = 1,
     ZCGVS_DTYPE_I8 = 2,
     ZCGVS_DTYPE_BINARY = 3,
-    ZCGVS_DTYPE_I8_ROW = 4
+    ZCGVS_DTYPE_I8_ROW = 4,
+    ZCGVS_DTYPE_BF16 = 5 /* bfloat16 values of the answer step; no corpus is stored in it */
 } zcgvs_dtype;
 
 /* Similarity metric; codes equal the reference Metric (include/zcgvs/core/metric.hpp:8-12).
@@ -423,6 +424,130 @@ int zcgvs_convert_i8_rows(const float* src, void* dst_int8, float* row_scales, i
 int zcgvs_pack_binary(const float* src, void* dst_words, int64_t rows, int dim, void* stream);
 int zcgvs_remap_indices(const int* candidates, const int* local_indices, int candidate_count,
                         int k, int batch, int* out_indices, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * The answer step: a language model that reads retrieved passages and answers keeps its keys and
+ * values in a paged cache, where passages that several requests read can share pages. One step
+ * takes the new tokens of a batch of sequences (a chunk of a passage or prompt, or the one token
+ * of a sequence that is being answered) and runs, in each layer, zcgvs_kv_append and
+ * zcgvs_paged_attention, and zcgvs_sample on the model's logits. The reference answers with an
+ * external runtime and has no counterpart of these entry points.
+ * --------------------------------------------------------------------------------------- */
+
+/* The cache of one layer: keys and values [pages, page_size, kv_heads, head_dim] of one type, in
+ * any order of the first three axes. Strides are in elements, the same for keys and values, and
+ * multiples of 8; both pointers are 16-byte aligned; head_dim is a multiple of 8, at most 128,
+ * and its elements are contiguous. */
+typedef struct zcgvs_paged_cache {
+    void* keys;
+    void* values;
+    int64_t pages;
+    int64_t page_stride;
+    int64_t slot_stride;
+    int64_t head_stride;
+    int page_size;
+    int kv_heads;
+    int head_dim;
+    int dtype; /* ZCGVS_DTYPE_F16 or ZCGVS_DTYPE_BF16 */
+} zcgvs_paged_cache;
+
+/* The new tokens of one step. Sequence s has the tokens [query_starts[s], query_starts[s + 1]) of
+ * the step's token rows; they are the last ones of its kv_lengths[s] cached tokens, so token j of
+ * n is at position kv_lengths[s] - n + j. Position p of sequence s lives in page
+ * page_table[s * page_table_stride + p / page_size], slot p % page_size. The three arrays are
+ * read on the device; query_starts must not decrease. A sequence may have no new token. Tokens
+ * at or past query_starts[sequences] (padding of a captured step) are ignored. Positions whose
+ * column is past pages_per_sequence do not exist; pages outside [0, pages) are never written, and
+ * read as zeros.
+ * max_new and max_length are the host's bounds of a sequence's new and cached tokens; they choose
+ * kernels and do not have to be tight, but max_new has to hold for the speed of long chunks. */
+typedef struct zcgvs_step_batch {
+    const int* query_starts; /* [sequences + 1] */
+    const int* kv_lengths;   /* [sequences], the new tokens included */
+    const int* page_table;   /* [sequences, pages_per_sequence] */
+    int64_t page_table_stride;
+    int pages_per_sequence;
+    int sequences;
+    int tokens; /* token rows of q, k, v and out */
+    int max_new;
+    int max_length;
+} zcgvs_step_batch;
+
+/* Norms and rotates the queries and keys of a step's new tokens and stores its keys and values in
+ * the paged cache, in one pass (all arithmetic in fp32, one rounding at the end):
+ *   1. where q_norm (k_norm) is given, every head x of a query (key) becomes
+ *      x * rsqrt(mean(x^2) + eps) * weight, the weights [head_dim] in the values' type;
+ *   2. where rotary is given, pair i of the first rotary_dim elements of a head, (x[i],
+ *      x[i + rotary_dim / 2]) or with `interleaved` (x[2 i], x[2 i + 1]), is turned by row p of
+ *      rotary [rotary_rows, rotary_dim] fp32 (rotary_dim / 2 cosines, then as many sines): (a, b) ->
+ *      (a cos - b sin, b cos + a sin). p is positions[token], or the token's cache position where
+ *      positions is NULL. rotary_dim is a multiple of 16, at most head_dim;
+ *   3. queries go to q_out (which may be q itself with the same strides), keys and values to the
+ *      token's slot.
+ * q, k, v and q_out are [tokens, heads, head_dim] rows of the cache's type with strides in
+ * elements (multiples of 8) and 16-byte aligned pointers, so that they may be views of one
+ * projection's rows. q may be NULL (q_heads 0): keys and values alone. k and v may be NULL
+ * together: queries alone, for a cache that already holds the step's keys.
+ * A token whose rotation row lies outside [0, rotary_rows) writes zeros to q_out and stores
+ * nothing; one whose cache position is negative or has no page stores nothing. Two tokens must
+ * not have the same slot. */
+int zcgvs_kv_append(const zcgvs_paged_cache* cache, const zcgvs_step_batch* batch, const void* q,
+                    int64_t q_token_stride, int64_t q_head_stride, int q_heads, const void* k,
+                    int64_t k_token_stride, int64_t k_head_stride, const void* v,
+                    int64_t v_token_stride, int64_t v_head_stride, const void* q_norm,
+                    const void* k_norm, float eps, const float* rotary, int64_t rotary_rows,
+                    int rotary_dim, int interleaved, const int* positions, void* q_out,
+                    int64_t q_out_token_stride, int64_t q_out_head_stride, void* stream);
+
+/* Attention of a step's new tokens over the paged cache (which already holds their keys and
+ * values). Query head h reads key/value head h / (q_heads / kv_heads). The token at position p
+ * sees the cached positions j < kv_lengths[s], with `causal` also j <= p, with window > 0 also
+ * j > p - window:
+ *   out = sum_j softmax_j(scale * q . k_j) v_j      lse = ln sum_j exp(scale * q . k_j)
+ * A token that sees nothing gets out = 0, lse = -inf. Scores, the softmax's running maximum and
+ * sum and the output are held in fp32; the weights are rounded to the values' type for the
+ * product with the values, as the tensor cores take them. Pages no token of the sequence sees are
+ * not read; slots at or past kv_lengths[s] may hold anything, NaN included.
+ *   q, out    : [tokens, q_heads, head_dim] in the cache's type, strides in elements (multiples of
+ *               8), 16-byte aligned.
+ *   lse       : optional fp32 [tokens, q_heads] (to join the result with attention over other
+ *               keys).
+ *   workspace : zcgvs_paged_attention_workspace_bytes() bytes, 256-byte aligned. Only its status
+ *               word (the first 4 bytes) must be zero before the first use; a non-zero word
+ *               afterwards (ZCGVS_DEVICE_*) means a bounded wait ran out. Calls that may overlap
+ *               need a workspace each.
+ * The result does not depend on timing: work is cut by the lengths alone and joined in order. */
+size_t zcgvs_paged_attention_workspace_bytes(int head_dim);
+
+int zcgvs_paged_attention(const zcgvs_paged_cache* cache, const zcgvs_step_batch* batch,
+                          const void* q, int64_t q_token_stride, int64_t q_head_stride, int q_heads,
+                          float scale, int causal, int window, void* out, int64_t out_token_stride,
+                          int64_t out_head_stride, float* lse, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
+/* Largest vocabulary of zcgvs_sample. */
+#define ZCGVS_MAX_VOCAB 327680
+
+/* Draws one token per row of logits [rows, vocab] (F32, F16 or BF16; row_stride elements apart)
+ * with one given uniform number in [0, 1) each. Tokens are ranked by (logit descending, id
+ * ascending). With m the largest logit of a row and t its temperature, token i weighs
+ *   w_i = rint(2^40 * exp((x_i - m) / t))
+ * whole units, so sums are exact and the draw depends on no order of summation. Kept are
+ *   top-k : the first top_k[row] ranked tokens (all when <= 0 or >= vocab);
+ *   top-p : of those, each whose predecessors weigh less than top_p[row] of their total (all when
+ *           >= 1; always the first);
+ *   min-p : of those, each with exp((x_i - m) / t) >= min_p[row] (all when <= 0; always the first).
+ * With Z the kept weight, the drawn token is the first in ascending id whose running kept weight
+ * exceeds min(floor(u * Z), Z - 1), products in fp64. temperature <= 0 (or NaN) takes the first
+ * ranked token. A logit of -inf or NaN is never drawn; one of +inf leaves only those; a row
+ * without any other gives token -1 and logprob -FLT_MAX.
+ *   temperature, top_k, top_p, min_p : [rows] on the device; NULL is 1, 0, 1 and 0 for all rows.
+ *   uniforms     : [rows]; values outside [0, 1) (NaN included) are clamped into it.
+ *   out_tokens   : [rows] int32.     out_logprobs : optional [rows] fp32, ln(w / Z) of the token.
+ * vocab is at most ZCGVS_MAX_VOCAB (ZCGVS_ERR_UNSUPPORTED beyond). */
+int zcgvs_sample(const void* logits, int dtype, int64_t row_stride, int rows, int vocab,
+                 const float* temperature, const int* top_k, const float* top_p, const float* min_p,
+                 const float* uniforms, int* out_tokens, float* out_logprobs, void* stream);
 
 #ifdef __cplusplus
 }  /* extern "C" */

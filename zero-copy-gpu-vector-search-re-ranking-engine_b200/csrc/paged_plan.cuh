@@ -1,0 +1,329 @@
+// How the attention kernels over the paged cache share a step's work among their CTAs.
+//
+// The rows of a sequence are its (new token, query head of one key/value head's group) pairs,
+// token major: row r is token r / group. They are cut into row tiles of R rows; a unit is one row
+// tile of one key/value head, and its cost is the number of KT-key tiles that any of its rows
+// sees (at least 1, so that rows that see nothing are written too). All key tiles of all units,
+// in the order (sequence, row tile, head, key tile), form one line; every CTA takes the same
+// number of consecutive key tiles of it, whatever the lengths, so all end together. A unit that
+// is cut between CTAs leaves one partial result per CTA (unnormalised sums, running maximum and
+// sum), and the CTA that finishes last joins them in the order of the CTAs: no CTA waits for
+// another, and the result does not depend on which one was last.
+//
+// Every CTA computes its own part of the line from the lengths on the device (about 2 us, no
+// launch of its own): a scan over the sequences, then a warp's scan over the row tiles of the
+// sequence where its part begins.
+#pragma once
+
+#include "common.cuh"
+#include "paged.h"
+
+namespace zc {
+namespace paged {
+
+struct AttnParams {
+    View view;
+    const uint8_t* q;
+    long long q_token, q_head;  // strides, elements
+    uint8_t* out;
+    long long out_token, out_head;
+    float* lse;  // optional [tokens, q_heads]
+    int q_heads;
+    int group;  // q_heads / kv_heads
+    float scale_log2;
+    int causal;
+    int window;
+    int rows_above;  // this kernel takes the sequences with rows_above < new tokens * group <= rows_to
+    int rows_to;
+    float* part_o;       // [2 per CTA][R][padded head_dim]
+    float* part_ml;      // [2 per CTA][R][2]: running maximum (log2 units) and sum
+    u64* tickets;        // [CTA]
+    uint32_t epoch;      // of this launch: a ticket of another epoch counts as zero
+    uint32_t* status;
+};
+
+struct Sequence {
+    int begin, n, length;
+};
+
+// Held within the step's rows, whatever the arrays say, so that no row outside them is touched.
+__device__ __forceinline__ Sequence load_sequence(const View& v, int s) {
+    const int begin = min(max(__ldg(v.starts + s), 0), v.tokens);
+    const int end = min(max(__ldg(v.starts + s + 1), begin), v.tokens);
+    return {begin, end - begin, max(__ldg(v.lengths + s), 0)};
+}
+
+// Keys [lo, hi) that some row of a row tile sees, and the tile's first key tile and count.
+struct UnitRange {
+    int lo, hi;
+    int first, count;
+};
+
+template <int R, int KT>
+__device__ __forceinline__ UnitRange unit_range(const AttnParams& p, const Sequence& q, int rt) {
+    const int rows = q.n * p.group;
+    const int r0 = rt * R, r1 = min(rows, r0 + R) - 1;
+    const int before = q.length - q.n;  // position of token 0
+    const int p0 = before + r0 / p.group, p1 = before + r1 / p.group;
+    const int cap = static_cast<int>(min(static_cast<long long>(q.length), static_cast<long long>(p.view.table_cols) * p.view.page_size));
+    UnitRange u;
+    u.hi = p1 < 0 ? 0 : (p.causal ? min(cap, p1 + 1) : cap);
+    u.lo = p.window > 0 && p0 >= p.window ? p0 - p.window + 1 : 0;
+    if (u.hi <= u.lo) u.lo = u.hi = 0;
+    u.first = u.lo / KT;
+    u.count = u.hi > u.lo ? (u.hi - 1) / KT - u.first + 1 : 1;
+    return u;
+}
+
+// Keys [lo, hi) that row r of a sequence sees.
+__device__ __forceinline__ void row_range(const AttnParams& p, const Sequence& q, int row, int cap, int& lo, int& hi) {
+    const int pos = q.length - q.n + row / p.group;
+    hi = pos < 0 ? 0 : (p.causal ? min(cap, pos + 1) : cap);
+    lo = p.window > 0 && pos >= p.window ? pos - p.window + 1 : 0;
+}
+
+// A CTA's stay at one unit: key tiles [begin, end) of the unit's `count`.
+struct Segment {
+    Sequence seq;
+    int s, rt, head;
+    UnitRange range;
+    int begin, end;
+    long long unit_start;  // the unit's first key tile on the line
+};
+
+constexpr int kCachedSequences = 512;
+
+template <int THREADS>
+struct PlanShared {
+    long long warp_sum[THREADS / 32];
+    long long found_before;
+    int found;
+    Segment segment;
+    int3 cached[kCachedSequences];
+    long long count[THREADS];
+};
+
+// GROUP lanes add up the row tiles of one sequence: 1 where sequences have few row tiles, 32
+// where they may have hundreds.
+template <int R, int KT, int THREADS, int GROUP>
+struct Planner {
+    const AttnParams& p;
+    PlanShared<THREADS>& sh;
+    long long total = 0;  // key tiles on the line
+    long long quota = 0;  // key tiles per CTA
+    long long at = 0, end = 0;  // this CTA's part that is left
+
+    __device__ Planner(const AttnParams& params, PlanShared<THREADS>& shared) : p(params), sh(shared) {}
+
+    __device__ __forceinline__ Sequence sequence(int s) const {
+        if (s < kCachedSequences) return {sh.cached[s].x, sh.cached[s].y, sh.cached[s].z};
+        return load_sequence(p.view, s);
+    }
+
+    __device__ __forceinline__ bool mine(const Sequence& q) const {
+        const long long rows = static_cast<long long>(q.n) * p.group;
+        return rows > p.rows_above && rows <= p.rows_to;
+    }
+
+    __device__ __forceinline__ int row_tiles(const Sequence& q) const { return (q.n * p.group + R - 1) / R; }
+
+    __device__ long long sequence_tiles(const Sequence& q, int lane) const {
+        if (!mine(q)) return 0;
+        long long sum = 0;
+        const int tiles = row_tiles(q);
+        for (int rt = lane; rt < tiles; rt += GROUP) sum += unit_range<R, KT>(p, q, rt).count;
+        return sum * p.view.kv_heads;
+    }
+
+    // Key tiles of sequence base + threadIdx.x (0 past the last); every thread calls it.
+    __device__ long long chunk_tiles(int base) const {
+        const int tid = threadIdx.x;
+        const int left = min(THREADS, p.view.sequences - base);
+        if constexpr (GROUP == 1) {
+            return tid < left ? sequence_tiles(sequence(base + tid), 0) : 0;
+        } else {
+            for (int i = tid >> 5; i < left; i += THREADS / 32) {
+                long long c = sequence_tiles(sequence(base + i), tid & 31);
+                for (int o = 16; o >= 1; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
+                if ((tid & 31) == 0) sh.count[i] = c;
+            }
+            __syncthreads();
+            const long long mine_count = tid < left ? sh.count[tid] : 0;
+            __syncthreads();
+            return mine_count;
+        }
+    }
+
+    // Inclusive sum of `c` over the CTA's threads; `all` gets the whole sum.
+    __device__ long long scan(long long c, long long& all) const {
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long t = __shfl_up_sync(0xffffffffu, c, o);
+            if (lane >= o) c += t;
+        }
+        __syncthreads();
+        if (lane == 31) sh.warp_sum[warp] = c;
+        __syncthreads();
+        all = 0;
+        for (int w = 0; w < THREADS / 32; ++w) {
+            const long long t = sh.warp_sum[w];
+            if (w < warp) c += t;
+            all += t;
+        }
+        return c;
+    }
+
+    // Finds this CTA's part of the line and its first segment. False when the CTA has none.
+    __device__ bool start(int least) {
+        const int tid = threadIdx.x;
+        const int sequences = p.view.sequences;
+        for (int s = tid; s < min(sequences, kCachedSequences); s += THREADS) {
+            const Sequence q = load_sequence(p.view, s);
+            sh.cached[s] = make_int3(q.begin, q.n, q.length);
+        }
+        __syncthreads();
+        long long c = 0, upto = 0, all = 0;
+        for (int base = 0; base < sequences; base += THREADS) {
+            c = chunk_tiles(base);
+            upto = scan(c, all);
+            total += all;
+        }
+        quota = max((total + gridDim.x - 1) / gridDim.x, static_cast<long long>(least));
+        at = quota * blockIdx.x;
+        end = min(total, at + quota);
+        if (at >= end) return false;
+        long long before = 0;
+        for (int base = 0; base < sequences; base += THREADS) {
+            if (sequences > THREADS) {  // else the values of the only chunk are still here
+                c = chunk_tiles(base);
+                upto = scan(c, all);
+            }
+            if (at >= before + upto - c && at < before + upto) {
+                sh.found = base + tid;
+                sh.found_before = before + upto - c;
+            }
+            before += all;
+            if (at < before) break;
+        }
+        __syncthreads();
+        if (tid < 32) {
+            Segment g;
+            g.s = sh.found;
+            g.seq = sequence(g.s);
+            long long rest = at - sh.found_before;
+            const int tiles = row_tiles(g.seq);
+            for (int base = 0; base < tiles; base += 32) {
+                const int rt = base + tid;
+                UnitRange u{};
+                if (rt < tiles) u = unit_range<R, KT>(p, g.seq, rt);
+                const long long cost = static_cast<long long>(u.count) * p.view.kv_heads;
+                long long sum = cost;
+                for (int o = 1; o < 32; o <<= 1) {
+                    const long long t = __shfl_up_sync(0xffffffffu, sum, o);
+                    if (tid >= o) sum += t;
+                }
+                const uint32_t over = __ballot_sync(0xffffffffu, rt < tiles && sum > rest);
+                if (over != 0u) {
+                    if (tid == __ffs(over) - 1) {
+                        const long long in = rest - (sum - cost);
+                        g.rt = rt;
+                        g.range = u;
+                        g.head = static_cast<int>(in / u.count);
+                        g.begin = static_cast<int>(in % u.count);
+                        g.end = static_cast<int>(min(static_cast<long long>(u.count), g.begin + (end - at)));
+                        g.unit_start = at - g.begin;
+                        sh.segment = g;
+                    }
+                    break;
+                }
+                rest -= __shfl_sync(0xffffffffu, sum, 31);
+            }
+        }
+        __syncthreads();
+        return true;
+    }
+
+    // Moves on to the CTA's next segment, after `done`. False when there is none. Only thread 0's
+    // shared copy is written; callers synchronise before they read it.
+    __device__ bool next(const Segment& done, Segment& g) {
+        at += done.end - done.begin;
+        if (at >= end) return false;
+        g = done;
+        if (++g.head == p.view.kv_heads) {
+            g.head = 0;
+            if (++g.rt >= row_tiles(g.seq)) {
+                g.rt = 0;
+                do {
+                    g.seq = sequence(++g.s);
+                } while (!mine(g.seq));
+            }
+            g.range = unit_range<R, KT>(p, g.seq, g.rt);
+        }
+        g.begin = 0;
+        g.end = static_cast<int>(min(static_cast<long long>(g.range.count), end - at));
+        g.unit_start = at;
+        return true;
+    }
+
+    // The partial slot of CTA c's stay at a unit: a CTA leaves at most two, its first segment's
+    // and its last one's.
+    __device__ __forceinline__ int slot(long long c, long long unit_start) const {
+        return static_cast<int>(2 * c + (unit_start <= c * quota ? 0 : 1));
+    }
+};
+
+// Counts the arrivals at one ticket; true for the last of `expected`, which leaves it at zero.
+__device__ __forceinline__ bool arrive_last(u64* ticket, uint32_t epoch, uint32_t expected) {
+    u64 seen = *reinterpret_cast<volatile u64*>(ticket);
+    for (;;) {
+        const uint32_t count = (seen >> 32) == epoch ? static_cast<uint32_t>(seen) + 1u : 1u;
+        const u64 next = count >= expected ? 0ull : (static_cast<u64>(epoch) << 32) | count;
+        const u64 old = atomicCAS(ticket, seen, next);
+        if (old == seen) return count >= expected;
+        seen = old;
+    }
+}
+
+// Joins the partial results of a cut unit and writes its rows' output. Every thread of the CTA
+// that arrived last calls it. A thread takes 4 elements of a row.
+template <typename T, int R, int DP, int THREADS, typename PLAN>
+__device__ void join_partials(const AttnParams& p, const PLAN& plan, const Segment& g) {
+    const int rows = min(R, g.seq.n * p.group - g.rt * R);
+    const long long c_first = g.unit_start / plan.quota, c_last = (g.unit_start + g.range.count - 1) / plan.quota;
+    constexpr int kPer = DP / 4;
+    for (int i = threadIdx.x; i < rows * kPer; i += THREADS) {
+        const int r = i / kPer, d = (i % kPer) * 4;
+        float top = -INFINITY;
+        for (long long c = c_first; c <= c_last; ++c) {
+            top = fmaxf(top, __ldcg(p.part_ml + (static_cast<long long>(plan.slot(c, g.unit_start)) * R + r) * 2));
+        }
+        const float base = top == -INFINITY ? 0.0f : top;
+        float sum = 0.0f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (long long c = c_first; c <= c_last; ++c) {
+            const long long at = static_cast<long long>(plan.slot(c, g.unit_start)) * R + r;
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml + at * 2));
+            const float4 part = __ldcg(reinterpret_cast<const float4*>(p.part_o + at * DP + d));
+            const float w = exp2f(ml.x - base);
+            sum += w * ml.y;
+            o.x += w * part.x;
+            o.y += w * part.y;
+            o.z += w * part.z;
+            o.w += w * part.w;
+        }
+        const int row = g.rt * R + r;
+        const int token = g.seq.begin + row / p.group, head = g.head * p.group + row % p.group;
+        const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
+        if (d < p.view.head_dim) {
+            const uint2 y = make_uint2(pack2<T>(o.x * inv, o.y * inv), pack2<T>(o.z * inv, o.w * inv));
+            *reinterpret_cast<uint2*>(p.out + 2 * (token * p.out_token + head * p.out_head + d)) = y;
+        }
+        if (d == 0 && p.lse != nullptr) {
+            p.lse[static_cast<long long>(token) * p.q_heads + head] = sum > 0.0f ? (base + log2f(sum)) * 0.69314718056f : (sum == 0.0f ? -INFINITY : sum);
+        }
+    }
+}
+
+}  // namespace paged
+}  // namespace zc

@@ -26,9 +26,10 @@ _DEVICE_STATUS_TEXT = {
     DEVICE_TMEM_WAIT_TIMEOUT: "a tensor-memory accumulator hand-off ran out",
     DEVICE_CANDIDATE_OVERFLOW: "a query kept more candidates than its buffer holds (its top-k is incomplete)",
 }
-DTYPE_F32, DTYPE_F16, DTYPE_I8, DTYPE_BINARY, DTYPE_I8_ROW = 0, 1, 2, 3, 4
+DTYPE_F32, DTYPE_F16, DTYPE_I8, DTYPE_BINARY, DTYPE_I8_ROW, DTYPE_BF16 = 0, 1, 2, 3, 4, 5
 METRIC_COSINE, METRIC_DOT, METRIC_L2 = 0, 1, 2
 MAX_K = 1024
+MAX_VOCAB = 327680
 
 _P = ctypes.c_void_p
 _i32, _i64, _f32, _sz = ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_size_t
@@ -84,6 +85,11 @@ SIGNATURES = {
     "zcgvs_bm25": (_i32, [_P, _P, _P, _P, _i32, _i32, _P, _P]),
     "zcgvs_max_positive": (_i32, [_P, _i32, _P, _P]),
     "zcgvs_fuse_scores": (_i32, [_P, _P, _P, _f32, _i32, _P]),
+    "zcgvs_kv_append": (_i32, [_P, _P, _P, _i64, _i64, _i32, _P, _i64, _i64, _P, _i64, _i64, _P, _P, _f32, _P, _i64,
+                               _i32, _i32, _P, _P, _i64, _i64, _P]),
+    "zcgvs_paged_attention_workspace_bytes": (_sz, [_i32]),
+    "zcgvs_paged_attention": (_i32, [_P, _P, _P, _i64, _i64, _i32, _f32, _i32, _i32, _P, _i64, _i64, _P, _P, _sz, _P]),
+    "zcgvs_sample": (_i32, [_P, _i32, _i64, _i32, _i32, _P, _P, _P, _P, _P, _P, _P, _P]),
 }
 
 
@@ -585,4 +591,207 @@ def pack_binary(src, out=None, stream=None):
     if out is None:
         out = torch.empty((rows, (dim + 31) // 32), dtype=torch.int32, device=src.device)
     check(lib().zcgvs_pack_binary(_ptr(src), _ptr(out), rows, dim, _stream(stream)))
+    return out
+
+
+# ------------------------------------------------------------------------------------------
+# The answer step: paged key/value cache, attention over it, sampling.
+# ------------------------------------------------------------------------------------------
+class _PagedCacheStruct(ctypes.Structure):
+    _fields_ = [("keys", _P), ("values", _P), ("pages", _i64), ("page_stride", _i64), ("slot_stride", _i64),
+                ("head_stride", _i64), ("page_size", _i32), ("kv_heads", _i32), ("head_dim", _i32), ("dtype", _i32)]
+
+
+class _StepBatchStruct(ctypes.Structure):
+    _fields_ = [("query_starts", _P), ("kv_lengths", _P), ("page_table", _P), ("page_table_stride", _i64),
+                ("pages_per_sequence", _i32), ("sequences", _i32), ("tokens", _i32), ("max_new", _i32),
+                ("max_length", _i32)]
+
+
+def _refuse(message: str):
+    raise InvalidArgument(ERR_INVALID_ARG, message)
+
+
+def _value_dtype(t, name: str, f32: bool = False) -> int:
+    import torch
+
+    code = {torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16, torch.float32: DTYPE_F32 if f32 else None}.get(t.dtype)
+    if code is None:
+        _refuse(f"{name}: unsupported type {t.dtype}")
+    return code
+
+
+def _on_device(device, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            _refuse(f"{name} is on {t.device}, not on {device}")
+
+
+def _typed(t, name: str, dtype, shape=None):
+    if t is None:
+        return
+    if t.dtype != dtype:
+        _refuse(f"{name} must be {dtype}, not {t.dtype}")
+    if not t.is_contiguous():
+        _refuse(f"{name} must be contiguous")
+    if shape is not None and tuple(t.shape) != shape:
+        _refuse(f"{name} must have shape {shape}, not {tuple(t.shape)}")
+
+
+class PagedKvCache:
+    """One layer's paged cache: `keys` and `values` are views [pages, page_size, kv_heads, head_dim]
+    of the caller's tensors (F16 or BF16), in any memory order of the first three axes."""
+
+    def __init__(self, keys, values):
+        if keys.dim() != 4 or keys.shape != values.shape or keys.stride() != values.stride() or keys.dtype != values.dtype:
+            _refuse("PagedKvCache: keys and values must be 4-D views of the same shape, strides and type")
+        if keys.shape[3] > 1 and keys.stride(3) != 1:
+            _refuse("PagedKvCache: the elements of a head must be contiguous")
+        _on_device(keys.device, values=values)
+        self.keys, self.values = keys, values
+        self.pages, self.page_size, self.kv_heads, self.head_dim = keys.shape
+        self.struct = _PagedCacheStruct(keys.data_ptr(), values.data_ptr(), self.pages, keys.stride(0), keys.stride(1),
+                                        keys.stride(2), self.page_size, self.kv_heads, self.head_dim,
+                                        _value_dtype(keys, "PagedKvCache"))
+        self.ref = ctypes.byref(self.struct)
+
+
+class StepBatch:
+    """The new tokens of one step over a paged cache (zcgvs_step_batch): int32 device tensors
+    query_starts [sequences + 1], kv_lengths [sequences] and page_table [sequences, pages], and the
+    host's bounds. `tokens` is the number of token rows; `max_new` and `max_length` bound one
+    sequence's new and cached tokens (default: any)."""
+
+    def __init__(self, query_starts, kv_lengths, page_table, *, tokens: int, max_new: int | None = None,
+                 max_length: int | None = None):
+        import torch
+
+        n = kv_lengths.numel()
+        _typed(query_starts, "query_starts", torch.int32, (n + 1,))
+        _typed(kv_lengths, "kv_lengths", torch.int32, (n,))
+        if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != n or \
+                (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+            _refuse("page_table must be int32 [sequences, pages] with contiguous rows")
+        _on_device(kv_lengths.device, query_starts=query_starts, page_table=page_table)
+        self.query_starts, self.kv_lengths, self.page_table = query_starts, kv_lengths, page_table
+        self.tokens, self.sequences = int(tokens), n
+        columns = page_table.shape[1]
+        stride = page_table.stride(0) if n > 1 else columns
+        self.struct = _StepBatchStruct(query_starts.data_ptr(), kv_lengths.data_ptr(), page_table.data_ptr(), stride,
+                                       columns, n, self.tokens, self.tokens if max_new is None else int(max_new),
+                                       2**31 - 1 if max_length is None else int(max_length))
+        self.ref = ctypes.byref(self.struct)
+
+
+def _rows(t, name: str, cache: PagedKvCache, batch: StepBatch, heads: int | None = None):
+    """(pointer, token stride, head stride) of a [tokens, heads, head_dim] operand."""
+    if t is None:
+        return None, 0, 0
+    if t.dim() != 3 or t.shape[0] != batch.tokens or t.shape[2] != cache.head_dim or (heads is not None and t.shape[1] != heads):
+        _refuse(f"{name} must be [{batch.tokens}, {heads if heads is not None else 'heads'}, {cache.head_dim}], "
+                f"not {tuple(t.shape)}")
+    if t.dtype != cache.keys.dtype:
+        _refuse(f"{name} must have the cache's type {cache.keys.dtype}, not {t.dtype}")
+    if cache.head_dim > 1 and t.stride(2) != 1:
+        _refuse(f"{name}: the elements of a head must be contiguous")
+    _on_device(cache.keys.device, **{name: t})
+    # The stride of an axis of one entry means nothing; 0 passes the library's checks.
+    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else 0, t.stride(1) if t.shape[1] > 1 else 0
+
+
+def rotary_table(rows: int, rotary_dim: int, base: float = 10000.0, device=None):
+    """The rotation table zcgvs_kv_append reads, [rows, rotary_dim] fp32 (cosines, then sines) of the
+    angles p * base^(-2 i / rotary_dim), computed in fp64 so that large positions stay exact."""
+    import torch
+
+    half = rotary_dim // 2
+    inv = base ** (-torch.arange(half, dtype=torch.float64) / half)
+    angle = torch.arange(rows, dtype=torch.float64)[:, None] * inv
+    return torch.cat([angle.cos(), angle.sin()], 1).float().to(device or "cuda")
+
+
+def kv_append(cache: PagedKvCache, batch: StepBatch, q, k, v, *, rotary=None, interleaved: bool = False, q_norm=None,
+              k_norm=None, eps: float = 1e-6, positions=None, out=None, stream=None):
+    """Norms and rotates a step's queries and keys [tokens, heads, head_dim] and stores its keys and
+    values in the paged cache. Returns the queries (`out`, which may be q), or None without q."""
+    import torch
+
+    device = cache.keys.device
+    _on_device(device, kv_lengths=batch.kv_lengths, rotary=rotary, q_norm=q_norm, k_norm=k_norm, positions=positions)
+    _typed(rotary, "rotary", torch.float32)
+    _typed(q_norm, "q_norm", cache.keys.dtype, (cache.head_dim,))
+    _typed(k_norm, "k_norm", cache.keys.dtype, (cache.head_dim,))
+    _typed(positions, "positions", torch.int32, (batch.tokens,))
+    if rotary is not None and rotary.dim() != 2:
+        _refuse("rotary must be [rows, rotary_dim]")
+    q_args = _rows(q, "q", cache, batch)
+    k_args = _rows(k, "k", cache, batch, cache.kv_heads)
+    v_args = _rows(v, "v", cache, batch, cache.kv_heads)
+    heads = 0 if q is None else q.shape[1]
+    if q is not None and out is None:
+        out = torch.empty((batch.tokens, heads, cache.head_dim), dtype=q.dtype, device=device)
+    o_args = _rows(out if q is not None else None, "out", cache, batch, heads)
+    rows, width = (0, 0) if rotary is None else rotary.shape
+    check(lib().zcgvs_kv_append(cache.ref, batch.ref, *q_args, heads, *k_args, *v_args, _ptr(q_norm), _ptr(k_norm), eps,
+                                _ptr(rotary), rows, width, 1 if interleaved else 0, _ptr(positions), *o_args,
+                                _stream(stream)))
+    return out if q is not None else None
+
+
+_attention_bytes: dict[tuple[int, int], int] = {}
+
+
+def paged_attention_workspace_bytes(head_dim: int) -> int:
+    return int(lib().zcgvs_paged_attention_workspace_bytes(head_dim))
+
+
+def paged_attention(cache: PagedKvCache, batch: StepBatch, q, *, scale: float, causal: bool = True, window: int = 0,
+                    return_lse: bool = False, workspace: Workspace | None = None, out=None, stream=None):
+    """Attention of a step's queries [tokens, q_heads, head_dim] over the paged cache. Returns the
+    output, with return_lse (output, fp32 [tokens, q_heads] log-sum-exp)."""
+    import torch
+
+    device = cache.keys.device
+    _on_device(device, kv_lengths=batch.kv_lengths)
+    if q is None:
+        _refuse("q must be given")
+    q_args = _rows(q, "q", cache, batch)
+    heads = q.shape[1]
+    if out is None:
+        out = torch.empty((batch.tokens, heads, cache.head_dim), dtype=q.dtype, device=device)
+    o_args = _rows(out, "out", cache, batch, heads)
+    lse = torch.empty((batch.tokens, heads), dtype=torch.float32, device=device) if return_lse else None
+    ws, owned = _own_workspace(workspace, device)
+    key = (device.index or 0, cache.head_dim)
+    nbytes = _attention_bytes.get(key)
+    if nbytes is None:
+        nbytes = _attention_bytes[key] = paged_attention_workspace_bytes(cache.head_dim)
+    buf = ws.get(nbytes, stream)
+    check(lib().zcgvs_paged_attention(cache.ref, batch.ref, *q_args, heads, scale, 1 if causal else 0, window, *o_args,
+                                      _ptr(lse), _ptr(buf), buf.numel(), _stream(stream)))
+    if owned:
+        ws.raise_on_status(stream)
+    return (out, lse) if return_lse else out
+
+
+def sample(logits, uniforms, *, temperature=None, top_k=None, top_p=None, min_p=None, out=None, stream=None):
+    """Draws one token per row of logits [rows, vocab] with the uniform numbers [rows]; temperature,
+    top_k (int32), top_p and min_p are [rows] device tensors or None. Returns (tokens int32 [rows],
+    logprobs fp32 [rows])."""
+    import torch
+
+    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        _refuse("logits must be [rows, vocab] with contiguous rows")
+    rows, vocab = logits.shape
+    dtype = _value_dtype(logits, "logits", f32=True)
+    for name, t in (("uniforms", uniforms), ("temperature", temperature), ("top_p", top_p), ("min_p", min_p)):
+        _typed(t, name, torch.float32, (rows,))
+    _typed(top_k, "top_k", torch.int32, (rows,))
+    _on_device(logits.device, uniforms=uniforms, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+    if out is None:
+        out = (torch.empty((rows,), dtype=torch.int32, device=logits.device),
+               torch.empty((rows,), dtype=torch.float32, device=logits.device))
+    check(lib().zcgvs_sample(_ptr(logits), dtype, logits.stride(0) if rows > 1 else vocab, rows, vocab, _ptr(temperature),
+                             _ptr(top_k), _ptr(top_p), _ptr(min_p), _ptr(uniforms), _ptr(out[0]), _ptr(out[1]),
+                             _stream(stream)))
     return out
