@@ -69,8 +69,8 @@ inline int make_view(const char* what, const zcgvs_paged_cache* cache, const zcg
     if (batch->pages_per_sequence <= 0 || batch->page_table_stride < batch->pages_per_sequence) {
         return invalid(what, "page_table_stride is smaller than pages_per_sequence, or that is not positive");
     }
-    if (static_cast<long long>(batch->pages_per_sequence) * cache->page_size > INT_MAX) {
-        return invalid(what, "pages_per_sequence * page_size exceeds 2^31 - 1 positions");
+    if (static_cast<long long>(batch->pages_per_sequence) * cache->page_size > INT_MAX - 1024) {
+        return invalid(what, "pages_per_sequence * page_size exceeds 2^31 - 1025 positions");
     }
     v.keys = static_cast<uint8_t*>(cache->keys);
     v.values = static_cast<uint8_t*>(cache->values);

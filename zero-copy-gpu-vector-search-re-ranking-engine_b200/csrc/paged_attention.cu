@@ -1,8 +1,17 @@
 // Host side of zcgvs_paged_attention: argument checks, the choice of kernels and the workspace.
+//
+// Two kernels share the sequences of a step by their rows (new tokens x group) per key/value head:
+// paged_stream.cuh takes those of at most 64 rows, which are bound by reading the cache, and
+// paged_chunk.cuh the longer ones, on the tensor cores. A step of one sequence, or one whose
+// sequences are all short, is one launch.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
 #include <algorithm>
 #include <atomic>
 #include <cmath>
 
+#include "paged_chunk.cuh"
 #include "paged_stream.cuh"
 
 namespace zc {
@@ -34,6 +43,14 @@ int padded(int head_dim) { return head_dim <= 64 ? 64 : 128; }
 constexpr int kStreamRows = 64;  // largest row tile of the streaming kernel
 
 int stream_ctas(int padded_dim, int sms) { return std::min(kMaxCtas, sms * (padded_dim == 64 ? stream_ctas_per_sm<64>() : stream_ctas_per_sm<128>())); }
+
+int chunk_ctas(int sms) { return std::min(kMaxCtas, sms); }
+
+static_assert(kStatusHandOff == ZCGVS_DEVICE_TMEM_WAIT_TIMEOUT, "device status bits must match the header");
+
+size_t workspace_rows(int padded_dim, int sms) {
+    return std::max(static_cast<size_t>(stream_ctas(padded_dim, sms)) * kStreamRows, static_cast<size_t>(chunk_ctas(sms)) * kChunkRows);
+}
 
 std::atomic<uint32_t> g_epoch{0};
 
@@ -68,6 +85,71 @@ cudaError_t launch_stream_any(const AttnParams& p, long long rows, int ctas, cud
                                          : launch_stream_rows<T, 128>(p, rows, ctas, stream);
 }
 
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+        void* ptr = nullptr;
+        cudaDriverEntryPointQueryResult found{};
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &found) != cudaSuccess ||
+            found != cudaDriverEntryPointSuccess) {
+            ptr = nullptr;
+        }
+        return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+    }();
+    return fn;
+}
+
+// Map of keys or values: (element, slot, head, page), boxes of 64 elements by `box` slots.
+// Elements past head_dim and pages out of range read as zeros.
+bool make_cache_map(CUtensorMap* map, void* base, const zcgvs_paged_cache& c, int box) {
+    const auto fn = encode_fn();
+    if (fn == nullptr) return false;
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(c.head_dim), static_cast<cuuint64_t>(c.page_size),
+                                static_cast<cuuint64_t>(c.kv_heads), static_cast<cuuint64_t>(c.pages)};
+    // The stride of an axis of one entry is never used, but must be a valid one.
+    const auto stride = [](int64_t elements, int64_t entries) { return static_cast<cuuint64_t>(entries > 1 ? 2 * elements : 16); };
+    const cuuint64_t strides[3] = {stride(c.slot_stride, c.page_size), stride(c.head_stride, c.kv_heads), stride(c.page_stride, c.pages)};
+    const cuuint32_t extent[4] = {64u, static_cast<cuuint32_t>(box), 1u, 1u};
+    const cuuint32_t step[4] = {1u, 1u, 1u, 1u};
+    return fn(map, c.dtype == ZCGVS_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, base, dims, strides,
+              extent, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+struct ChunkMaps {
+    CUtensorMap keys, values;
+    int box_log2 = 0;
+};
+
+// Whether the chunk kernel can take this cache: pages made of whole groups of 8 slots (the
+// swizzle's), and strides a tensor map accepts.
+bool make_chunk_maps(const zcgvs_paged_cache& c, ChunkMaps& maps) {
+    if (c.page_size % 8 != 0 || c.pages <= 0) return false;
+    int log2 = 3;
+    while (log2 < 7 && c.page_size % (2 << log2) == 0) ++log2;
+    maps.box_log2 = log2;
+    return make_cache_map(&maps.keys, c.keys, c, 1 << log2) && make_cache_map(&maps.values, c.values, c, 1 << log2);
+}
+
+template <typename T, int DP>
+cudaError_t launch_chunk(const AttnParams& base, const ChunkMaps& maps, int ctas, cudaStream_t stream) {
+    const auto kernel = chunk_kernel<T, DP>;
+    const cudaError_t e = ensure_smem_optin(reinterpret_cast<const void*>(kernel));
+    if (e != cudaSuccess) return e;
+    AttnParams p = base;
+    // The kernel takes a positive scale: a negative one turns the queries' signs, and zero becomes
+    // a number whose product with any finite score is zero in the exponent.
+    const uint32_t sign = p.scale_log2 < 0.0f ? 0x80008000u : 0u;
+    p.scale_log2 = std::max(std::fabs(p.scale_log2), 1e-37f);
+    KernelTimer timer("paged_chunk", stream);
+    kernel<<<ctas, kChunkThreads, chunk_smem_bytes<DP>(), stream>>>(maps.keys, maps.values, p, maps.box_log2, sign);
+    return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t launch_chunk_any(const AttnParams& p, const ChunkMaps& maps, int ctas, cudaStream_t stream) {
+    return padded(p.view.head_dim) == 64 ? launch_chunk<T, 64>(p, maps, ctas, stream) : launch_chunk<T, 128>(p, maps, ctas, stream);
+}
+
 }  // namespace
 }  // namespace paged
 }  // namespace zc
@@ -79,7 +161,7 @@ size_t zcgvs_paged_attention_workspace_bytes(int head_dim) {
     if (head_dim <= 0 || head_dim > kMaxHeadDim) return 0;
     const int dim = padded(head_dim);
     const size_t sms = static_cast<size_t>(zc::device_sm_count());
-    return layout(static_cast<size_t>(stream_ctas(dim, static_cast<int>(sms))) * kStreamRows, dim).total;
+    return layout(workspace_rows(dim, static_cast<int>(sms)), dim).total;
 }
 
 int zcgvs_paged_attention(const zcgvs_paged_cache* cache, const zcgvs_step_batch* batch, const void* q,
@@ -123,6 +205,7 @@ int zcgvs_paged_attention(const zcgvs_paged_cache* cache, const zcgvs_step_batch
     p.lse = lse;
     p.q_heads = q_heads;
     p.group = group;
+    p.by_group = Divider(static_cast<uint32_t>(group));
     p.scale_log2 = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);
     p.causal = causal != 0;
     p.window = window;
@@ -133,12 +216,25 @@ int zcgvs_paged_attention(const zcgvs_paged_cache* cache, const zcgvs_step_batch
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const long long rows = static_cast<long long>(std::min(batch->max_new, batch->tokens)) * group;
 
-    const int ctas = stream_ctas(dim, device_sm_count());
-    p.part_o = reinterpret_cast<float*>(ws + layout(static_cast<size_t>(ctas) * kStreamRows, dim).part_o);
+    const int sms = device_sm_count();
+    p.part_o = reinterpret_cast<float*>(ws + layout(workspace_rows(dim, sms), dim).part_o);
+    const bool f16 = cache->dtype == ZCGVS_DTYPE_F16;
     p.rows_above = 0;
     p.rows_to = INT_MAX;
-    const cudaError_t e = cache->dtype == ZCGVS_DTYPE_F16 ? launch_stream_any<__half>(p, rows, ctas, s)
-                                                          : launch_stream_any<__nv_bfloat16>(p, rows, ctas, s);
+    ChunkMaps maps;
+    if (rows > kStreamRows && make_chunk_maps(*cache, maps)) {
+        // One sequence goes to the chunk kernel whatever its length (max_new says it is long).
+        if (batch->sequences > 1) p.rows_above = kStreamRows;
+        const cudaError_t e = f16 ? launch_chunk_any<__half>(p, maps, chunk_ctas(sms), s) : launch_chunk_any<__nv_bfloat16>(p, maps, chunk_ctas(sms), s);
+        if (e != cudaSuccess) return fail_cuda(e, what);
+        if (batch->sequences == 1) return ok();
+        p.rows_above = 0;
+        p.rows_to = kStreamRows;
+        p.epoch = next_epoch();
+    }
+    const long long stream_rows = std::min(rows, static_cast<long long>(p.rows_to));
+    const int ctas = stream_ctas(dim, sms);
+    const cudaError_t e = f16 ? launch_stream_any<__half>(p, stream_rows, ctas, s) : launch_stream_any<__nv_bfloat16>(p, stream_rows, ctas, s);
     if (e != cudaSuccess) return fail_cuda(e, what);
     return ok();
 }

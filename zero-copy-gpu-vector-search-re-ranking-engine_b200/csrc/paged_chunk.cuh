@@ -1,0 +1,673 @@
+// Attention of many rows per sequence over the paged cache: chunks of prompts and passages, on the
+// fifth-generation tensor cores (tcgen05, TMEM, TMA).
+//
+// A unit is 256 rows of one key/value head, two halves of 128 that share every key and value tile
+// of 128 keys:
+//   * Warp 8 (producer) brings the tiles from their pages into a ring of shared-memory slots with
+//     4-D TMA loads (64 elements x the largest power of two of slots that a page holds whole, at
+//     most 128; 128-byte swizzle). Pages out of range read as zeros. Where a value tile is only
+//     partly inside the unit's keys, it clears the other rows itself before it hands the tile
+//     over: a weight of 0 times a NaN left in an unused slot would be a NaN.
+//   * Warp 9 (one thread) issues the products: S_h = Q_h K^T (both operands K-major in shared
+//     memory) and O_h += P_h V (P from tensor memory, V as it lies, MN-major), h = 0, 1. While
+//     the tensor cores work for one half, the softmax of the other runs.
+//   * Warps 0-3 and 4-7 (softmax of half 0 and 1; a thread holds a row) read a row's 128 scores
+//     from tensor memory, keep the running maximum and sum, and write the weights back over the
+//     scores in the values' type. The reference point of the exponentials is moved (and O
+//     rescaled, in tensor memory) only when the maximum rose by more than 8 in log2 units, so
+//     weights stay below 2^8 and rescaling is rare; the result is the same, since sum and O share
+//     the reference point.
+// Tensor memory: S_0, S_1 (P over them) and O_0, O_1, 128 columns each.
+//
+// Scores, maxima, sums and O are fp32. The weights are rounded to the cache's type, as the second
+// product takes both operands in one type.
+//
+// Every wait is bounded; on a timeout a status bit is set, all roles stop, copies and products in
+// flight are waited for (bounded) and tensor memory is freed.
+#pragma once
+
+#include <cuda.h>
+
+#include <type_traits>
+
+#include "paged_plan.cuh"
+
+namespace zc {
+namespace paged {
+
+constexpr int kChunkRows = 256;
+constexpr int kChunkKeys = 128;
+constexpr int kChunkThreads = 384;  // warps 10 and 11 only complete the third warpgroup
+constexpr int kProducerWarp = 8;
+constexpr int kIssueWarp = 9;
+constexpr int kSoftmaxThreads = 256;
+constexpr int kSoftmaxBarrier = 1;
+// Registers: the launch gives 168 to each of 384 threads (64,512); the softmax warpgroups hold a
+// row's 128 scores and take 208, the third gives up the difference: 256 * 208 + 128 * 88 = 64,512.
+constexpr int kSoftmaxRegisters = 208;
+constexpr int kOtherRegisters = 88;
+constexpr int kFmaOf8 = 2;  // of 8 pairs of weights, those computed by exp2_fma
+constexpr float kRescaleAbove = 8.0f;  // log2 units
+
+template <int DP>
+constexpr int chunk_slots() {
+    return DP == 128 ? 4 : 8;
+}
+template <int DP>
+constexpr int chunk_slot_bytes() {
+    return kChunkKeys * DP * 2;
+}
+template <int DP>
+constexpr int chunk_smem_bytes() {
+    return kChunkRows * DP * 2 + chunk_slots<DP>() * chunk_slot_bytes<DP>() + 1024;
+}
+
+enum : uint32_t { kStatusHandOff = 4u };  // ZCGVS_DEVICE_TMEM_WAIT_TIMEOUT
+
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// The issuing warp runs converged and its instructions carry the leader's predicate: operands then
+// stay in uniform registers, and a product costs a few issue slots instead of about a hundred
+// cycles (measured: 1,630 cycles for 16 products behind a one-thread branch).
+__device__ __forceinline__ void commit_to(u64* bar, uint32_t leader) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(smem_u32(bar)),
+        "r"(leader)
+        : "memory");
+}
+
+// Shared-memory descriptors, 128-byte swizzle: rows of 128 bytes in groups of 8 (1024 bytes). The
+// high word is the same for all: SBO 1024, version 1, the swizzle mode. In the low word lie the
+// address and LBO. K-major operands: groups along the rows follow at SBO, LBO is not used.
+// MN-major: K runs along the rows, groups of 8 at SBO, further 64-element columns at LBO.
+constexpr uint32_t kDescHigh = 64u | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_low(uint32_t addr, uint32_t lbo) { return ((addr >> 4) & 0x3FFFu) | ((lbo >> 4) << 16); }
+
+// fp32 accumulator, both operands of one 16-bit type, M = 128.
+template <typename T>
+__device__ __forceinline__ constexpr uint32_t instruction(int n, bool b_mn_major) {
+    constexpr uint32_t type = std::is_same<T, __half>::value ? 0u : 1u;  // f16, bf16
+    return (1u << 4) | (type << 7) | (type << 10) | (b_mn_major ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) |
+           (static_cast<uint32_t>(128 >> 4) << 24);
+}
+
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool accumulate, uint32_t leader) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "mov.b64 da, {%1, %6};\n\tmov.b64 db, {%2, %6};\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}\n" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(accumulate ? 1u : 0u), "r"(leader), "r"(kDescHigh));
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool accumulate, uint32_t leader) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 db;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "mov.b64 db, {%2, %6};\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}\n" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(accumulate ? 1u : 0u), "r"(leader), "r"(kDescHigh));
+}
+
+__device__ __forceinline__ void tmem_load32(uint32_t addr, float* v) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
+          "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]),
+          "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]),
+          "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+        : "r"(addr));
+}
+__device__ __forceinline__ void tmem_load_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t* v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
+        "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
+        "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_load16(uint32_t addr, float* v) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+                 : "r"(addr));
+}
+__device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t* v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// One box of a cache map: 64 elements from x, box slots from `slot`, one head, one page.
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int x, int slot, int head, int page, u64* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(slot), "r"(head), "r"(page), "r"(smem_u32(bar))
+        : "memory");
+}
+
+// Named barrier over the softmax warps that also ANDs a predicate across them.
+__device__ __forceinline__ bool softmax_barrier(bool pred) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\t"
+        "bar.red.and.pred q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(r)
+        : "r"(pred ? 1 : 0), "n"(kSoftmaxBarrier), "n"(kSoftmaxThreads)
+        : "memory");
+    return r != 0u;
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float y;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 ra, rb, rc, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\tmov.b64 rc, {%6, %7};\n\t"
+        "fma.rn.f32x2 rd, ra, rb, rc;\n\tmov.b64 {%0, %1}, rd;\n\t}\n"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 ra, rb, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
+        "add.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}\n"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
+// 2^x on the FMA units, for x <= 127 (below -126 as -126): x = n + f with n the nearest integer
+// (left in the low bits by adding 1.5 * 2^23) and a polynomial of degree 4 for 2^f on [-1/2, 1/2],
+// the minimax one of the relative error (own Remez exchange: 2.6e-6 at most, 1.4e-8 on average),
+// whose exponent n is added to. The special-function unit gives 16 results per cycle and SM, and
+// 128 x 128 of them take as long as both products of a tile; a part of them goes here instead.
+__device__ __forceinline__ float2 exp2_fma(float2 x) {
+    x = make_float2(fmaxf(x.x, -126.0f), fmaxf(x.y, -126.0f));
+    const float2 n = add2(x, both(12582912.0f));
+    const float2 f = add2(x, fma2(add2(n, both(-12582912.0f)), both(-1.0f), both(0.0f)));
+    float2 y = fma2(both(0.009570102207362652f), f, both(0.05591785907745361f));
+    y = fma2(y, f, both(0.240247443318367f));
+    y = fma2(y, f, both(0.6931217908859253f));
+    y = fma2(y, f, both(0.9999992847442627f));
+    return make_float2(__int_as_float(__float_as_int(y.x) + (__float_as_int(n.x) << 23)),
+                       __int_as_float(__float_as_int(y.y) + (__float_as_int(n.y) << 23)));
+}
+
+// Called by all warps of a warpgroup, first thing in its branch: a split before the branch would
+// bound both sides by the smaller number.
+__device__ __forceinline__ void give_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegisters)); }
+__device__ __forceinline__ void take_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters)); }
+
+struct ChunkShared {
+    u64 kv_full[8], kv_empty[8];
+    u64 raw;  // a value tile that the producer still has to clear rows of
+    u64 q_full[2], s_full[2], o_full[2];
+    u64 p_full[2][2];  // of each half, the weights of the tile's first and second 64 keys
+    u64 drain;
+    uint32_t tmem;
+    int abort;
+    int last;
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kChunkThreads, 1)
+    chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const AttnParams p, int box_log2,
+                 uint32_t q_sign) {
+    constexpr int kSlots = chunk_slots<DP>();
+    constexpr int kSlotBytes = chunk_slot_bytes<DP>();
+    constexpr int kHalves = DP / 64;                 // 64-element columns of a row
+    constexpr int kColumnBytes = kChunkKeys * 128;   // one of them, 128 rows
+    constexpr int kQBytes = 128 * DP * 2;            // one half of Q
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ PlanShared<kChunkThreads> plan_shared;
+    __shared__ ChunkShared sh;
+
+    const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t q_smem = smem;
+    const uint32_t kv_smem = smem + 2 * kQBytes;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const View& view = p.view;
+
+    Planner<kChunkRows, kChunkKeys, kChunkThreads, 32> plan(p, plan_shared);
+    if (!plan.start(4)) return;
+
+    if (tid == 0) {
+        for (int s = 0; s < kSlots; ++s) {
+            mbar_init(&sh.kv_full[s], 1);
+            mbar_init(&sh.kv_empty[s], 1);
+        }
+        mbar_init(&sh.raw, 1);
+        for (int h = 0; h < 2; ++h) {
+            mbar_init(&sh.q_full[h], 128);
+            mbar_init(&sh.s_full[h], 1);
+            mbar_init(&sh.p_full[h][0], 128);
+            mbar_init(&sh.p_full[h][1], 128);
+            mbar_init(&sh.o_full[h], 1);
+        }
+        mbar_init(&sh.drain, 1);
+        fence_mbarrier_init();
+        sh.abort = 0;
+    }
+    if (warp == kIssueWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = sh.tmem;
+    volatile int* abort_flag = &sh.abort;
+    Segment g = plan_shared.segment;
+
+    // Waits for a phase, or gives up for the whole CTA.
+    auto wait = [&](u64* bar, uint32_t parity, uint32_t flag) {
+        if (mbar_try_wait(smem_u32(bar), parity)) return true;
+        if (*abort_flag || !mbar_wait_bounded(bar, parity, p.status, flag)) {
+            *abort_flag = 1;
+            return false;
+        }
+        return true;
+    };
+
+    if (warp >= kProducerWarp) {
+    give_registers();
+    if (warp == kProducerWarp) {
+        // ---------------- producer ----------------
+        const int box = 1 << box_log2;
+        const int boxes = kChunkKeys >> box_log2;       // per tile and 64-element column
+        const uint32_t box_bytes = static_cast<uint32_t>(box) * 128u;
+        uint32_t used = 0;  // slots handed out
+        uint32_t raw_phase = 0;
+        bool ok = true;
+        for (bool more = true; more && ok;) {
+            for (int t = g.begin; t < g.end && ok; ++t) {
+                const int pos0 = (g.range.first + t) * kChunkKeys;
+                const bool partial = pos0 < g.range.lo || pos0 + kChunkKeys > g.range.hi;
+                // Lane i takes box i (and i + 32 where a tile has more than 32 boxes of a column: never, 128 / 8 = 16).
+                const int pos = pos0 + lane * box;
+                const bool mine = lane < boxes && pos < g.range.hi && pos + box > g.range.lo;
+                int page = -1, slot = 0;
+                if (mine) {
+                    const int column = page_column(view, pos);
+                    page = __ldg(view.table + g.s * view.table_stride + column);
+                    slot = pos - column * view.page_size;
+                }
+                const int count = __popc(__ballot_sync(0xffffffffu, mine));
+                for (int which = 0; which < 2 && ok; ++which) {  // the keys, then the values
+                    const int s = static_cast<int>(used % kSlots);
+                    if (used >= kSlots) ok = wait(&sh.kv_empty[s], ((used / kSlots) - 1u) & 1u, kStatusTileWaitTimeout);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    const bool clear = which == 1 && partial;
+                    u64* bar = clear ? &sh.raw : &sh.kv_full[s];
+                    const uint32_t dst = kv_smem + s * kSlotBytes;
+                    if (lane == 0) mbar_arrive_expect_tx(bar, static_cast<uint32_t>(count) * box_bytes * kHalves);
+                    __syncwarp();
+                    if (mine) {
+#pragma unroll
+                        for (int c = 0; c < kHalves; ++c) {
+                            load_box(dst + c * kColumnBytes + lane * box_bytes, which == 0 ? &map_k : &map_v, c * 64, slot, g.head, page, bar);
+                        }
+                    }
+                    ++used;
+                    if (clear) {
+                        // In flight on `raw` alone: waited for here, also when the others gave up.
+                        ok = mbar_wait_bounded(&sh.raw, raw_phase, p.status, kStatusTileWaitTimeout);
+                        raw_phase ^= 1u;
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) {
+                            *abort_flag = 1;
+                            break;
+                        }
+                        const int a = max(g.range.lo - pos0, 0), b = min(max(g.range.hi - pos0, 0), kChunkKeys);
+                        for (int i = lane; i < kChunkKeys * 8 * kHalves; i += 32) {
+                            const int row = (i >> 3) & (kChunkKeys - 1);
+                            if (row < a || row >= b) {
+                                const uint32_t at = dst + (i >> 3) * 128 + (i & 7) * 16;
+                                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
+                            }
+                        }
+                        fence_proxy_async_shared();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_cta(&sh.kv_full[s]);
+                    }
+                }
+            }
+            Segment following;
+            more = plan.next(g, following);
+            g = following;
+        }
+        if (*abort_flag) {
+            // Copies in flight land before the CTA retires. Slots of cleared tiles have completed already.
+            for (uint32_t i = used > kSlots ? used - kSlots : 0; i < used; ++i) {
+                mbar_wait_bounded(&sh.kv_full[i % kSlots], (i / kSlots) & 1u, p.status, kStatusDrainTimeout);
+            }
+        }
+    } else if (warp == kIssueWarp) {
+        // ---------------- products ----------------
+        constexpr uint32_t kScores = instruction<T>(kChunkKeys, false);
+        constexpr uint32_t kOutput = instruction<T>(DP, true);
+        const uint32_t leader = lane == 0 ? 1u : 0u;
+        uint32_t used = 0;               // slots consumed
+        uint32_t step[2] = {0u, 0u};     // tiles of each half, over all segments
+        uint32_t segments[2] = {0u, 0u};
+        bool ok = true;
+        auto slot_full = [&](uint32_t i) {
+            return __all_sync(0xffffffffu, wait(&sh.kv_full[i % kSlots], (i / kSlots) & 1u, kStatusTileWaitTimeout)) != 0;
+        };
+        auto scores = [&](int h, uint32_t slot) {
+            fence_after();
+            const uint32_t a = desc_low(q_smem + h * kQBytes, 16), b = desc_low(kv_smem + (slot % kSlots) * kSlotBytes, 16);
+#pragma unroll
+            for (int kk = 0; kk < DP / 16; ++kk) {
+                const uint32_t at = ((kk >> 2) * kColumnBytes + (kk & 3) * 32) >> 4;
+                mma_ss(tmem + h * 128, a + at, b + at, kScores, kk > 0, leader);
+            }
+            commit_to(&sh.s_full[h], leader);
+        };
+        auto output = [&](int h, uint32_t slot, int part, bool first) {
+            fence_after();
+            const uint32_t b = desc_low(kv_smem + (slot % kSlots) * kSlotBytes, kColumnBytes);
+#pragma unroll
+            for (int i = 0; i < kChunkKeys / 32; ++i) {
+                const int kk = part * (kChunkKeys / 32) + i;
+                mma_ts(tmem + 256 + h * 128, tmem + h * 128 + kk * 8, b + ((kk * 2048) >> 4), kOutput, !first || kk > 0, leader);
+            }
+        };
+        for (bool more = true; more && ok;) {
+            const int halves = g.seq.n * p.group - g.rt * kChunkRows > 128 ? 2 : 1;
+            const int tiles = g.end - g.begin;
+            // Slots of this segment: keys of tile t at used + 2 t, values at used + 2 t + 1.
+            ok = slot_full(used);
+            for (int h = 0; h < halves && ok; ++h) {
+                ok = __all_sync(0xffffffffu, wait(&sh.q_full[h], segments[h] & 1u, kStatusHandOff));
+                ++segments[h];
+                if (ok) scores(h, used);
+            }
+            if (ok) commit_to(&sh.kv_empty[used % kSlots], leader);
+            for (int t = 0; t < tiles && ok; ++t) {
+                const uint32_t values = used + 2 * t + 1, keys = values + 1;
+                ok = slot_full(values);
+                for (int h = 0; h < halves && ok; ++h) {
+                    for (int part = 0; part < 2 && ok; ++part) {
+                        ok = __all_sync(0xffffffffu, wait(&sh.p_full[h][part], step[h] & 1u, kStatusHandOff));
+                        if (ok) output(h, values, part, t == 0);
+                    }
+                    ++step[h];
+                    if (!ok) break;
+                    commit_to(&sh.o_full[h], leader);
+                    if (h == halves - 1) commit_to(&sh.kv_empty[values % kSlots], leader);
+                    if (t + 1 < tiles) {
+                        if (h == 0) ok = slot_full(keys);
+                        if (!ok) break;
+                        scores(h, keys);
+                        if (h == halves - 1) commit_to(&sh.kv_empty[keys % kSlots], leader);
+                    }
+                }
+            }
+            used += 2 * tiles;
+            Segment following;
+            more = plan.next(g, following);
+            g = following;
+        }
+        // No product is in flight when tensor memory is freed.
+        commit_to(&sh.drain, leader);
+        mbar_wait_bounded(&sh.drain, 0u, p.status, kStatusDrainTimeout);
+    }
+    } else {
+        // ---------------- softmax ----------------
+        take_registers();
+        const int h = warp >> 2;
+        const int r = tid & 127;  // row of the half = TMEM lane
+        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const uint32_t s_addr = tmem + lanes + h * 128;
+        const uint32_t o_addr = tmem + lanes + 256 + h * 128;
+        const float scale = p.scale_log2;
+        uint32_t step = 0;  // tiles of this half, over all segments
+
+        // Brings the rows of this half of a unit to shared memory, 16 bytes per thread and row; all
+        // loads of a batch are in flight together.
+        auto load_queries = [&](const Segment& of) {
+            constexpr int kPieces = DP / 8, kStep = 128 / kPieces, kBatch = 8;
+            const int rows = of.seq.n * p.group - of.rt * kChunkRows - h * 128;  // live ones
+            const int piece = r % kPieces, row0 = r / kPieces;
+            const bool inside = piece * 8 < view.head_dim;
+#pragma unroll
+            for (int b = 0; b < 128 / kStep; b += kBatch) {
+                uint4 v[kBatch];
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i) {
+                    const int rr = row0 + (b + i) * kStep;
+                    const int global = of.rt * kChunkRows + h * 128 + rr;
+                    const int j = p.by_group.quotient(global);
+                    const long long token = of.seq.begin + j;
+                    const int head = of.head * p.group + global - j * p.group;
+                    v[i] = make_uint4(0u, 0u, 0u, 0u);
+                    if (rr < rows && inside) v[i] = __ldg(reinterpret_cast<const uint4*>(p.q + 2 * (token * p.q_token + head * p.q_head + piece * 8)));
+                }
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i) {
+                    const int rr = row0 + (b + i) * kStep;
+                    const uint32_t at = q_smem + h * kQBytes + (piece >> 3) * kColumnBytes + rr * 128 + (((piece & 7) ^ (rr & 7)) << 4);
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v[i].x ^ q_sign), "r"(v[i].y ^ q_sign),
+                                 "r"(v[i].z ^ q_sign), "r"(v[i].w ^ q_sign)
+                                 : "memory");
+                }
+            }
+            fence_proxy_async_shared();
+            mbar_arrive_cta(&sh.q_full[h]);
+        };
+        auto half_works = [&](const Segment& of) { return h == 0 || of.seq.n * p.group - of.rt * kChunkRows > 128; };
+
+        if (half_works(g)) load_queries(g);
+        for (bool more = true; more;) {
+            const int rows = g.seq.n * p.group - g.rt * kChunkRows;  // live rows of the unit, if below 256
+            const bool works = half_works(g);
+            const bool whole_unit = g.begin == 0 && g.end == g.range.count;
+            const int row = g.rt * kChunkRows + h * 128 + r;  // of the sequence
+            const bool live = h * 128 + r < rows;
+            bool ok = true;
+            float top = -INFINITY, sum = 0.0f;  // reference point (raw score units), sum of weights
+            if (works) {
+                const int cap = static_cast<int>(min(static_cast<long long>(g.seq.length), static_cast<long long>(view.table_cols) * view.page_size));
+                int lo, hi;
+                row_range(p, g.seq, row, cap, lo, hi);
+                if (!live) lo = hi = 0;
+                // A tile inside the range of every live row of the warp needs no mask; padding rows'
+                // queries are zeros and their results are dropped.
+                const int all_lo = __reduce_max_sync(0xffffffffu, live ? lo : 0), all_hi = __reduce_min_sync(0xffffffffu, live ? hi : INT_MAX);
+
+                for (int t = g.begin; t < g.end && ok; ++t, ++step) {
+                    ok = __all_sync(0xffffffffu, wait(&sh.s_full[h], step & 1u, kStatusHandOff));
+                    if (!ok) break;
+                    fence_after();
+                    float s[128];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) tmem_load32(s_addr + c * 32, s + c * 32);
+                    tmem_load_wait();
+                    const int pos0 = (g.range.first + t) * kChunkKeys;
+                    const bool masked = pos0 < all_lo || pos0 + kChunkKeys > all_hi;
+                    if (masked) {
+                        const int a = lo - pos0;
+                        const uint32_t n = static_cast<uint32_t>(max(hi - lo, 0));
+#pragma unroll
+                        for (int c = 0; c < 128; ++c) s[c] = static_cast<uint32_t>(c - a) < n ? s[c] : -INFINITY;
+                    }
+                    float m[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                    for (int c = 4; c + 8 <= 128; c += 8) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) m[i] = max3(m[i], s[c + 2 * i], s[c + 2 * i + 1]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) m[i] = fmaxf(m[i], s[124 + i]);
+                    const float best = fmaxf(max3(m[0], m[1], m[2]), m[3]);
+                    float shrink = 1.0f;
+                    if (top == -INFINITY) {
+                        // Nothing seen yet: sum and this row of O are zero.
+                        top = best;
+                    } else if ((best - top) * scale > kRescaleAbove) {
+                        shrink = exp2_fast((top - best) * scale);
+                        top = best;
+                    }
+                    if (__any_sync(0xffffffffu, shrink != 1.0f)) {
+                        // O holds the tiles before this one; its last product must be done. (t >
+                        // g.begin here: top was -inf at the first.)
+                        ok = __all_sync(0xffffffffu, wait(&sh.o_full[h], (step - 1u) & 1u, kStatusHandOff));
+                        if (!ok) break;
+                        fence_after();
+#pragma unroll 1
+                        for (int c = 0; c < DP; c += 16) {
+                            float o[16];
+                            tmem_load16(o_addr + c, o);
+                            tmem_load_wait();
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) o[i] *= shrink;
+                            tmem_store16(o_addr + c, reinterpret_cast<const uint32_t*>(o));
+                        }
+                        sum *= shrink;
+                    }
+                    const float2 base2 = both(top == -INFINITY ? 0.0f : -top * scale), scale2 = both(scale);
+                    float2 part[2] = {both(0.0f), both(0.0f)};
+                    // Each half of the keys is handed over as soon as its weights are written.
+                    auto weigh = [&](auto fma_of_8, int from) {
+                        uint32_t packed[32];
+#pragma unroll
+                        for (int c = 0; c < 64; c += 2) {
+                            const float2 x = fma2(make_float2(s[from + c], s[from + c + 1]), scale2, base2);
+                            float2 w;
+                            if ((c >> 1) % 8 < fma_of_8) {
+                                w = exp2_fma(x);
+                            } else {
+                                w = make_float2(exp2_fast(x.x), exp2_fast(x.y));
+                            }
+                            part[(c >> 1) & 1] = add2(part[(c >> 1) & 1], w);
+                            packed[c >> 1] = pack2<T>(w.x, w.y);
+                        }
+                        tmem_store32(s_addr + from / 2, packed);
+                        tmem_store_wait();
+                        fence_before();
+                        mbar_arrive_cta(&sh.p_full[h][from / 64]);
+                    };
+                    if (masked) {  // exp2_fma gives no zero
+                        weigh(std::integral_constant<int, 0>{}, 0);
+                        weigh(std::integral_constant<int, 0>{}, 64);
+                    } else {
+                        weigh(std::integral_constant<int, kFmaOf8>{}, 0);
+                        weigh(std::integral_constant<int, kFmaOf8>{}, 64);
+                    }
+                    part[0] = add2(part[0], part[1]);
+                    sum += part[0].x + part[0].y;
+                }
+            }
+            Segment following;
+            more = plan.next(g, following);
+            if (ok && more) {
+                // The products that read this half's queries are done (its last scores were waited
+                // for), so the next unit's scores can start while this one's output is written. A
+                // half that did not work in this unit was waited for in an earlier one.
+                if (half_works(following)) load_queries(following);
+            }
+            if (works && ok) {
+                // The unit's rows, or this CTA's part of them.
+                ok = __all_sync(0xffffffffu, wait(&sh.o_full[h], (step - 1u) & 1u, kStatusHandOff));
+            }
+            if (works && ok) {
+                fence_after();
+                const float base = top == -INFINITY ? 0.0f : top * scale;
+                const int j = p.by_group.quotient(row);
+                const long long token = g.seq.begin + j;
+                const int head = g.head * p.group + row - j * p.group;
+                const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
+                uint8_t* out = p.out + 2 * (token * p.out_token + head * p.out_head);
+                const long long at = static_cast<long long>(plan.slot(blockIdx.x, g.unit_start)) * kChunkRows + h * 128 + r;
+                float* part = p.part_o + at * DP;
+#pragma unroll 1
+                for (int c = 0; c < DP; c += 32) {
+                    float o[32];
+                    tmem_load32(o_addr + c, o);
+                    tmem_load_wait();
+                    if (!live) continue;
+                    if (whole_unit) {
+#pragma unroll
+                        for (int i = 0; i < 32; i += 8) {
+                            if (c + i < view.head_dim) {
+                                *reinterpret_cast<uint4*>(out + 2 * (c + i)) =
+                                    make_uint4(pack2<T>(o[i] * inv, o[i + 1] * inv), pack2<T>(o[i + 2] * inv, o[i + 3] * inv),
+                                               pack2<T>(o[i + 4] * inv, o[i + 5] * inv), pack2<T>(o[i + 6] * inv, o[i + 7] * inv));
+                            }
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(part + c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                    }
+                }
+                if (live && whole_unit && p.lse != nullptr) {
+                    p.lse[token * p.q_heads + head] = sum > 0.0f ? (base + log2f(sum)) * 0.69314718056f : (sum == 0.0f ? -INFINITY : sum);
+                }
+                if (live && !whole_unit) {
+                    *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(top == -INFINITY ? top : base, sum);
+                }
+                fence_before();  // O is read before the next unit's products overwrite it (after this thread's next arrival)
+            }
+            if (!whole_unit) {
+                __threadfence();
+                ok = softmax_barrier(ok);
+                if (ok) {
+                    if (tid == 0) {
+                        const long long c_first = g.unit_start / plan.quota, c_last = (g.unit_start + g.range.count - 1) / plan.quota;
+                        sh.last = arrive_last(p.tickets + c_first, p.epoch, static_cast<uint32_t>(c_last - c_first + 1)) ? 1 : 0;
+                    }
+                    softmax_barrier(true);
+                    if (sh.last) {
+                        __threadfence();
+                        join_partials<T, kChunkRows, DP, kSoftmaxThreads>(p, plan, g);
+                    }
+                    softmax_barrier(true);  // sh.last is read before it is written again
+                }
+            }
+            if (!ok) {
+                *abort_flag = 1;
+                // The other softmax warps meet at the next cut unit's barrier: end it for them too.
+                bool met = !whole_unit;
+                while (!met && more) {
+                    g = following;
+                    met = g.begin != 0 || g.end != g.range.count;
+                    if (met) {
+                        softmax_barrier(false);
+                    } else {
+                        more = plan.next(g, following);
+                    }
+                }
+                break;
+            }
+            g = following;
+        }
+    }
+
+    fence_before();
+    __syncthreads();
+    fence_after();
+    if (warp == kIssueWarp) {
+        __syncwarp();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+}  // namespace paged
+}  // namespace zc

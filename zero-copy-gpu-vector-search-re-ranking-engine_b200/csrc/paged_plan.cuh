@@ -21,6 +21,21 @@
 namespace zc {
 namespace paged {
 
+// Division of a number below 2^31 by a fixed one: a high product, an addition and a shift.
+struct Divider {
+    uint32_t magic = 1;
+    int shift = 0;
+
+    Divider() = default;
+    explicit Divider(uint32_t d) {
+        while ((1ull << shift) < d) ++shift;
+        magic = static_cast<uint32_t>(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
+    }
+    __device__ __forceinline__ int quotient(int n) const {
+        return static_cast<int>((__umulhi(static_cast<uint32_t>(n), magic) + static_cast<uint32_t>(n)) >> shift);
+    }
+};
+
 struct AttnParams {
     View view;
     const uint8_t* q;
@@ -30,6 +45,7 @@ struct AttnParams {
     float* lse;  // optional [tokens, q_heads]
     int q_heads;
     int group;  // q_heads / kv_heads
+    Divider by_group;
     float scale_log2;
     int causal;
     int window;
@@ -64,7 +80,7 @@ __device__ __forceinline__ UnitRange unit_range(const AttnParams& p, const Seque
     const int rows = q.n * p.group;
     const int r0 = rt * R, r1 = min(rows, r0 + R) - 1;
     const int before = q.length - q.n;  // position of token 0
-    const int p0 = before + r0 / p.group, p1 = before + r1 / p.group;
+    const int p0 = before + p.by_group.quotient(r0), p1 = before + p.by_group.quotient(r1);
     const int cap = static_cast<int>(min(static_cast<long long>(q.length), static_cast<long long>(p.view.table_cols) * p.view.page_size));
     UnitRange u;
     u.hi = p1 < 0 ? 0 : (p.causal ? min(cap, p1 + 1) : cap);
@@ -77,7 +93,7 @@ __device__ __forceinline__ UnitRange unit_range(const AttnParams& p, const Seque
 
 // Keys [lo, hi) that row r of a sequence sees.
 __device__ __forceinline__ void row_range(const AttnParams& p, const Sequence& q, int row, int cap, int& lo, int& hi) {
-    const int pos = q.length - q.n + row / p.group;
+    const int pos = q.length - q.n + p.by_group.quotient(row);
     hi = pos < 0 ? 0 : (p.causal ? min(cap, pos + 1) : cap);
     lo = p.window > 0 && pos >= p.window ? pos - p.window + 1 : 0;
 }
@@ -285,42 +301,88 @@ __device__ __forceinline__ bool arrive_last(u64* ticket, uint32_t epoch, uint32_
 }
 
 // Joins the partial results of a cut unit and writes its rows' output. Every thread of the CTA
-// that arrived last calls it. A thread takes 4 elements of a row.
+// that arrived last calls it (THREADS of them, by tid). A warp takes 4 rows at a time, so that
+// their loads are in flight together; its lanes first hold the maxima and sums of up to 32 CTAs
+// each, then DP / 32 elements of the rows. The sums run in the order of the CTAs.
 template <typename T, int R, int DP, int THREADS, typename PLAN>
 __device__ void join_partials(const AttnParams& p, const PLAN& plan, const Segment& g) {
+    constexpr int kRows = 4, kWarps = THREADS / 32, kPer = DP / 32;
     const int rows = min(R, g.seq.n * p.group - g.rt * R);
-    const long long c_first = g.unit_start / plan.quota, c_last = (g.unit_start + g.range.count - 1) / plan.quota;
-    constexpr int kPer = DP / 4;
-    for (int i = threadIdx.x; i < rows * kPer; i += THREADS) {
-        const int r = i / kPer, d = (i % kPer) * 4;
-        float top = -INFINITY;
-        for (long long c = c_first; c <= c_last; ++c) {
-            top = fmaxf(top, __ldcg(p.part_ml + (static_cast<long long>(plan.slot(c, g.unit_start)) * R + r) * 2));
+    const long long c_first = g.unit_start / plan.quota;
+    const int parts = static_cast<int>((g.unit_start + g.range.count - 1) / plan.quota - c_first) + 1;
+    const int lane = threadIdx.x & 31;
+    const auto at = [&](int c, int row) { return static_cast<long long>(plan.slot(c_first + c, g.unit_start)) * R + row; };
+    for (int first = threadIdx.x >> 5; first < rows; first += kWarps * kRows) {
+        float base[kRows], sum[kRows], o[kRows][kPer];
+        int row[kRows];
+#pragma unroll
+        for (int u = 0; u < kRows; ++u) {
+            row[u] = min(first + u * kWarps, rows - 1);
+            base[u] = -INFINITY;
+            sum[u] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) o[u][i] = 0.0f;
         }
-        const float base = top == -INFINITY ? 0.0f : top;
-        float sum = 0.0f;
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-        for (long long c = c_first; c <= c_last; ++c) {
-            const long long at = static_cast<long long>(plan.slot(c, g.unit_start)) * R + r;
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml + at * 2));
-            const float4 part = __ldcg(reinterpret_cast<const float4*>(p.part_o + at * DP + d));
-            const float w = exp2f(ml.x - base);
-            sum += w * ml.y;
-            o.x += w * part.x;
-            o.y += w * part.y;
-            o.z += w * part.z;
-            o.w += w * part.w;
+        for (int c = lane; c < parts; c += 32) {
+#pragma unroll
+            for (int u = 0; u < kRows; ++u) base[u] = fmaxf(base[u], __ldcg(p.part_ml + at(c, row[u]) * 2));
         }
-        const int row = g.rt * R + r;
-        const int token = g.seq.begin + row / p.group, head = g.head * p.group + row % p.group;
-        const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
-        if (d < p.view.head_dim) {
-            const uint2 y = make_uint2(pack2<T>(o.x * inv, o.y * inv), pack2<T>(o.z * inv, o.w * inv));
-            *reinterpret_cast<uint2*>(p.out + 2 * (token * p.out_token + head * p.out_head + d)) = y;
+#pragma unroll
+        for (int u = 0; u < kRows; ++u) {
+            base[u] = warp_max_f32(base[u]);
+            if (base[u] == -INFINITY) base[u] = 0.0f;
         }
-        if (d == 0 && p.lse != nullptr) {
-            p.lse[static_cast<long long>(token) * p.q_heads + head] = sum > 0.0f ? (base + log2f(sum)) * 0.69314718056f : (sum == 0.0f ? -INFINITY : sum);
+        for (int c0 = 0; c0 < parts; c0 += 32) {
+            float w[kRows], l[kRows];
+#pragma unroll
+            for (int u = 0; u < kRows; ++u) {
+                float2 ml = make_float2(-INFINITY, 0.0f);
+                if (c0 + lane < parts) ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml + at(c0 + lane, row[u]) * 2));
+                w[u] = exp2f(ml.x - base[u]);
+                l[u] = w[u] * ml.y;
+            }
+            const int n = min(32, parts - c0);
+#pragma unroll 2
+            for (int c = 0; c < n; ++c) {
+#pragma unroll
+                for (int u = 0; u < kRows; ++u) {
+                    const float* src = p.part_o + at(c0 + c, row[u]) * DP + lane * kPer;
+                    const float f = __shfl_sync(0xffffffffu, w[u], c);
+                    sum[u] += __shfl_sync(0xffffffffu, l[u], c);
+                    if constexpr (kPer == 4) {
+                        const float4 v = __ldcg(reinterpret_cast<const float4*>(src));
+                        o[u][0] += f * v.x;
+                        o[u][1] += f * v.y;
+                        o[u][2] += f * v.z;
+                        o[u][3] += f * v.w;
+                    } else {
+                        const float2 v = __ldcg(reinterpret_cast<const float2*>(src));
+                        o[u][0] += f * v.x;
+                        o[u][1] += f * v.y;
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kRows; ++u) {
+            if (first + u * kWarps >= rows) continue;
+            const int of = g.rt * R + row[u];
+            const int j = p.by_group.quotient(of);
+            const long long token = g.seq.begin + j;
+            const int head = g.head * p.group + of - j * p.group;
+            const float inv = sum[u] > 0.0f ? 1.0f / sum[u] : (sum[u] == 0.0f ? 0.0f : sum[u]);
+            if (lane * kPer < p.view.head_dim) {
+                uint8_t* dst = p.out + 2 * (token * p.out_token + head * p.out_head + lane * kPer);
+                if constexpr (kPer == 4) {
+                    *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(o[u][0] * inv, o[u][1] * inv), pack2<T>(o[u][2] * inv, o[u][3] * inv));
+                } else {
+                    *reinterpret_cast<uint32_t*>(dst) = pack2<T>(o[u][0] * inv, o[u][1] * inv);
+                }
+            }
+            if (lane == 0 && p.lse != nullptr) {
+                p.lse[token * p.q_heads + head] =
+                    sum[u] > 0.0f ? (base[u] + log2f(sum[u])) * 0.69314718056f : (sum[u] == 0.0f ? -INFINITY : sum[u]);
+            }
         }
     }
 }

@@ -160,8 +160,9 @@ __global__ void __launch_bounds__(kStreamThreads, stream_ctas_per_sm<DP>()) stre
             const bool live = row < rows;
             row_range(p, g.seq, row, cap, lo[h], hi[h]);
             if (!live) hi[h] = 0;
-            const long long token = g.seq.begin + row / p.group;
-            const int head = g.head * p.group + row % p.group;
+            const int j = p.by_group.quotient(row);
+            const long long token = g.seq.begin + j;
+            const int head = g.head * p.group + row - j * p.group;
             const uint8_t* src = p.q + 2 * (token * p.q_token + head * p.q_head);
 #pragma unroll
             for (int kk = 0; kk < DP / 16; ++kk) {
@@ -330,8 +331,9 @@ __global__ void __launch_bounds__(kStreamThreads, stream_ctas_per_sm<DP>()) stre
             }
             if (whole_unit) {
                 const int row = g.rt * R + r;
-                const long long token = g.seq.begin + row / p.group;
-                const int head = g.head * p.group + row % p.group;
+                const int j = p.by_group.quotient(row);
+                const long long token = g.seq.begin + j;
+                const int head = g.head * p.group + row - j * p.group;
                 const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
                 if (d < view.head_dim) {
                     *reinterpret_cast<uint2*>(p.out + 2 * (token * p.out_token + head * p.out_head + d)) =
