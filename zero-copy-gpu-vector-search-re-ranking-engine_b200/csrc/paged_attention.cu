@@ -2,8 +2,8 @@
 //
 // Two kernels share the sequences of a step by their rows (new tokens x group) per key/value head:
 // paged_stream.cuh takes those of at most 64 rows, which are bound by reading the cache, and
-// paged_chunk.cuh the longer ones, on the tensor cores. A step of one sequence, or one whose
-// sequences are all short, is one launch.
+// paged_chunk.cuh the longer ones, on the tensor cores (behind it a small kernel joins units that
+// were cut). A step whose sequences are all short is one launch.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -19,11 +19,14 @@ namespace paged {
 
 namespace {
 
-// Workspace: the status word, then a ticket per CTA, then two partial results per CTA. Sized for
-// the largest grid and row tile of any variant.
+// Workspace: the status word, a ticket per CTA (stream kernel), a cut unit's description per CTA
+// (chunk kernel), two partial results per CTA. Sized for the largest grid and row tile of any
+// variant; the kernels of a call use it one after the other.
 constexpr int kMaxCtas = 1024;
 constexpr size_t kTicketsAt = 256;
-constexpr size_t kPartMlAt = kTicketsAt + sizeof(u64) * kMaxCtas;
+constexpr size_t kJoinsAt = kTicketsAt + sizeof(u64) * kMaxCtas;
+constexpr size_t kPartMlAt = kJoinsAt + sizeof(Join) * kMaxCtas;
+static_assert(kPartMlAt % 16 == 0, "partial results are read 16 bytes at a time");
 
 struct Layout {
     size_t part_o;
@@ -115,14 +118,30 @@ bool make_cache_map(CUtensorMap* map, void* base, const zcgvs_paged_cache& c, in
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Map of the queries: (element, head, token), boxes of 64 elements by a head group by as many
+// tokens as make 128 rows.
+bool make_query_map(CUtensorMap* map, const AttnParams& p, int dtype) {
+    const auto fn = encode_fn();
+    if (fn == nullptr) return false;
+    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(p.view.head_dim), static_cast<cuuint64_t>(p.q_heads), static_cast<cuuint64_t>(p.view.tokens)};
+    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(p.q_heads > 1 ? 2 * p.q_head : 16), static_cast<cuuint64_t>(p.view.tokens > 1 ? 2 * p.q_token : 16)};
+    const cuuint32_t extent[3] = {64u, static_cast<cuuint32_t>(p.group), static_cast<cuuint32_t>(128 / p.group)};
+    const cuuint32_t step[3] = {1u, 1u, 1u};
+    return fn(map, dtype == ZCGVS_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<uint8_t*>(p.q), dims,
+              strides, extent, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 struct ChunkMaps {
-    CUtensorMap keys, values;
+    CUtensorMap keys, values, queries;
     int box_log2 = 0;
+    int q_by_tma = 0;
 };
 
 // Whether the chunk kernel can take this cache: pages made of whole groups of 8 slots (the
 // swizzle's), and strides a tensor map accepts.
-bool make_chunk_maps(const zcgvs_paged_cache& c, ChunkMaps& maps) {
+bool make_chunk_maps(const zcgvs_paged_cache& c, const AttnParams& p, ChunkMaps& maps) {
+    maps.q_by_tma = (p.group & (p.group - 1)) == 0 && p.group <= 128 && make_query_map(&maps.queries, p, c.dtype) ? 1 : 0;
     if (c.page_size % 8 != 0 || c.pages <= 0) return false;
     int log2 = 3;
     while (log2 < 7 && c.page_size % (2 << log2) == 0) ++log2;
@@ -136,13 +155,30 @@ cudaError_t launch_chunk(const AttnParams& base, const ChunkMaps& maps, int ctas
     const cudaError_t e = ensure_smem_optin(reinterpret_cast<const void*>(kernel));
     if (e != cudaSuccess) return e;
     AttnParams p = base;
-    // The kernel takes a positive scale: a negative one turns the queries' signs, and zero becomes
-    // a number whose product with any finite score is zero in the exponent.
-    const uint32_t sign = p.scale_log2 < 0.0f ? 0x80008000u : 0u;
-    p.scale_log2 = std::max(std::fabs(p.scale_log2), 1e-37f);
-    KernelTimer timer("paged_chunk", stream);
-    kernel<<<ctas, kChunkThreads, chunk_smem_bytes<DP>(), stream>>>(maps.keys, maps.values, p, maps.box_log2, sign);
-    return cudaGetLastError();
+    // Masked scores are -inf times the scale in the exponent: a scale of 0 becomes a number whose
+    // product with any finite score is 0 there.
+    p.scale_log2 = std::max(p.scale_log2, 1e-37f);
+    Join* joins = reinterpret_cast<Join*>(reinterpret_cast<uint8_t*>(p.status) + kJoinsAt);
+    {
+        KernelTimer timer("paged_chunk", stream);
+        kernel<<<ctas, kChunkThreads, chunk_smem_bytes<DP>(), stream>>>(maps.keys, maps.values, maps.q_by_tma ? maps.queries : maps.keys, p, joins,
+                                                                       maps.box_log2, maps.q_by_tma);
+    }
+    cudaError_t launched = cudaGetLastError();
+    if (launched != cudaSuccess) return launched;
+    // The joins wait for the chunk kernel on the device (griddepcontrol.wait); only their launch
+    // overlaps with it.
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(static_cast<unsigned>(ctas), kChunkRows / kJoinRows);
+    config.blockDim = dim3(kJoinThreads);
+    config.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = attr;
+    config.numAttrs = 1;
+    KernelTimer timer("paged_join", stream);
+    return cudaLaunchKernelEx(&config, join_kernel<T, DP>, p, static_cast<const Join*>(joins));
 }
 
 template <typename T>
@@ -222,7 +258,7 @@ int zcgvs_paged_attention(const zcgvs_paged_cache* cache, const zcgvs_step_batch
     p.rows_above = 0;
     p.rows_to = INT_MAX;
     ChunkMaps maps;
-    if (rows > kStreamRows && make_chunk_maps(*cache, maps)) {
+    if (rows > kStreamRows && p.scale_log2 >= 0.0f && make_chunk_maps(*cache, p, maps)) {
         // One sequence goes to the chunk kernel whatever its length (max_new says it is long).
         if (batch->sequences > 1) p.rows_above = kStreamRows;
         const cudaError_t e = f16 ? launch_chunk_any<__half>(p, maps, chunk_ctas(sms), s) : launch_chunk_any<__nv_bfloat16>(p, maps, chunk_ctas(sms), s);

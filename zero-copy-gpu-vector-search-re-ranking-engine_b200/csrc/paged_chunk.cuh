@@ -8,9 +8,11 @@
 //     most 128; 128-byte swizzle). Pages out of range read as zeros. Where a value tile is only
 //     partly inside the unit's keys, it clears the other rows itself before it hands the tile
 //     over: a weight of 0 times a NaN left in an unused slot would be a NaN.
-//   * Warp 9 (one thread) issues the products: S_h = Q_h K^T (both operands K-major in shared
-//     memory) and O_h += P_h V (P from tensor memory, V as it lies, MN-major), h = 0, 1. While
-//     the tensor cores work for one half, the softmax of the other runs.
+//   * Warps 9 and 10 issue the products of half 0 and 1: S_h = Q_h K^T (both operands K-major in
+//     shared memory) and O_h += P_h V (P from tensor memory, V as it lies, MN-major). While the
+//     tensor cores work for one half, the softmax of the other runs. A warp of its own for each
+//     half, as the tensor cores queue only about two instructions: a warp that waits for one
+//     half's weights would hold up the other's products.
 //   * Warps 0-3 and 4-7 (softmax of half 0 and 1; a thread holds a row) read a row's 128 scores
 //     from tensor memory, keep the running maximum and sum, and write the weights back over the
 //     scores in the values' type. The reference point of the exponentials is moved (and O
@@ -37,11 +39,9 @@ namespace paged {
 
 constexpr int kChunkRows = 256;
 constexpr int kChunkKeys = 128;
-constexpr int kChunkThreads = 384;  // warps 10 and 11 only complete the third warpgroup
+constexpr int kChunkThreads = 384;  // warp 11 only completes the third warpgroup
 constexpr int kProducerWarp = 8;
-constexpr int kIssueWarp = 9;
-constexpr int kSoftmaxThreads = 256;
-constexpr int kSoftmaxBarrier = 1;
+constexpr int kIssueWarp = 9;  // and 10
 // Registers: the launch gives 168 to each of 384 threads (64,512); the softmax warpgroups hold a
 // row's 128 scores and take 208, the third gives up the difference: 256 * 208 + 128 * 88 = 64,512.
 constexpr int kSoftmaxRegisters = 208;
@@ -57,9 +57,11 @@ template <int DP>
 constexpr int chunk_slot_bytes() {
     return kChunkKeys * DP * 2;
 }
+constexpr int kStageBytes = 32 * 64;  // a softmax warp's output on its way out: 32 rows of 32 elements
+
 template <int DP>
 constexpr int chunk_smem_bytes() {
-    return kChunkRows * DP * 2 + chunk_slots<DP>() * chunk_slot_bytes<DP>() + 1024;
+    return kChunkRows * DP * 2 + chunk_slots<DP>() * chunk_slot_bytes<DP>() + 8 * kStageBytes + 1024;
 }
 
 enum : uint32_t { kStatusHandOff = 4u };  // ZCGVS_DEVICE_TMEM_WAIT_TIMEOUT
@@ -141,23 +143,17 @@ __device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t* v) {
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // One box of a cache map: 64 elements from x, box slots from `slot`, one head, one page.
+__device__ __forceinline__ void load_queries_box(uint32_t dst, const CUtensorMap* map, int x, int head, int token, u64* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(head), "r"(token), "r"(smem_u32(bar))
+        : "memory");
+}
 __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int x, int slot, int head, int page, u64* bar) {
     asm volatile(
         "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
         "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(slot), "r"(head), "r"(page), "r"(smem_u32(bar))
         : "memory");
-}
-
-// Named barrier over the softmax warps that also ANDs a predicate across them.
-__device__ __forceinline__ bool softmax_barrier(bool pred) {
-    uint32_t r;
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\t"
-        "bar.red.and.pred q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-        : "=r"(r)
-        : "r"(pred ? 1 : 0), "n"(kSoftmaxBarrier), "n"(kSoftmaxThreads)
-        : "memory");
-    return r != 0u;
 }
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -216,18 +212,33 @@ __device__ __forceinline__ void take_registers() { asm volatile("setmaxnreg.inc.
 struct ChunkShared {
     u64 kv_full[8], kv_empty[8];
     u64 raw;  // a value tile that the producer still has to clear rows of
-    u64 q_full[2], s_full[2], o_full[2];
+    u64 q_full[2], q_empty[2], s_full[2], o_full[2];
     u64 p_full[2][2];  // of each half, the weights of the tile's first and second 64 keys
-    u64 drain;
+    u64 drain[2];
     uint32_t tmem;
     int abort;
-    int last;
 };
+
+// A unit that was cut, written by the CTA where it starts: join_kernel reads one per CTA.
+struct Join {
+    int begin;  // of the sequence: its first token
+    int n;      // its new tokens
+    int rt, head;
+    int first_slot;  // the first CTA's partial; those of the next ones are their first, 2 * CTA
+    int parts;       // 0: none
+};
+
+// Partial results of the chunk kernel: [slot][DP / 4][256 rows][4], so that a warp's 32 rows write
+// and read 512 bytes at a time.
+template <int DP>
+__device__ __forceinline__ long long part_at(long long slot, int column4, int row) {
+    return ((slot * (DP / 4) + column4) * kChunkRows + row) * 4;
+}
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(kChunkThreads, 1)
-    chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const AttnParams p, int box_log2,
-                 uint32_t q_sign) {
+    chunk_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_q,
+                 const AttnParams p, Join* joins, int box_log2, int q_by_tma) {
     constexpr int kSlots = chunk_slots<DP>();
     constexpr int kSlotBytes = chunk_slot_bytes<DP>();
     constexpr int kHalves = DP / 64;                 // 64-element columns of a row
@@ -240,26 +251,33 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t q_smem = smem;
     const uint32_t kv_smem = smem + 2 * kQBytes;
+    const uint32_t stage_smem = kv_smem + kSlots * kSlotBytes;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const View& view = p.view;
 
     Planner<kChunkRows, kChunkKeys, kChunkThreads, 32> plan(p, plan_shared);
-    if (!plan.start(4)) return;
+    if (!plan.start(4)) {
+        if (tid == 0) joins[blockIdx.x].parts = 0;
+        return;
+    }
 
     if (tid == 0) {
+        joins[blockIdx.x].parts = 0;
         for (int s = 0; s < kSlots; ++s) {
             mbar_init(&sh.kv_full[s], 1);
-            mbar_init(&sh.kv_empty[s], 1);
+            mbar_init(&sh.kv_empty[s], 2);  // both issuing warps
         }
         mbar_init(&sh.raw, 1);
         for (int h = 0; h < 2; ++h) {
-            mbar_init(&sh.q_full[h], 128);
+            mbar_init(&sh.q_full[h], q_by_tma ? 1 : 128);
+            mbar_init(&sh.q_empty[h], 1);
             mbar_init(&sh.s_full[h], 1);
             mbar_init(&sh.p_full[h][0], 128);
             mbar_init(&sh.p_full[h][1], 128);
             mbar_init(&sh.o_full[h], 1);
         }
-        mbar_init(&sh.drain, 1);
+        mbar_init(&sh.drain[0], 1);
+        mbar_init(&sh.drain[1], 1);
         fence_mbarrier_init();
         sh.abort = 0;
     }
@@ -293,19 +311,58 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         const uint32_t box_bytes = static_cast<uint32_t>(box) * 128u;
         uint32_t used = 0;  // slots handed out
         uint32_t raw_phase = 0;
+        uint32_t queries[2] = {0u, 0u};  // loads of each half's queries
         bool ok = true;
+        // Lane i takes box i of a tile (at most 16). Its page is looked up one tile ahead.
+        struct Box {
+            bool mine;
+            int page, slot;
+        };
+        auto find = [&](const Segment& of, int t) {
+            const int pos = (of.range.first + t) * kChunkKeys + lane * box;
+            Box b{lane < boxes && pos < of.range.hi && pos + box > of.range.lo, -1, 0};
+            if (b.mine) {
+                const int column = page_column(view, pos);
+                b.page = __ldg(view.table + of.s * view.table_stride + column);
+                b.slot = pos - column * view.page_size;
+            }
+            return b;
+        };
+        Box ahead = find(g, g.begin);
         for (bool more = true; more && ok;) {
+            Segment following;
+            more = plan.next(g, following);
+            if (q_by_tma) {
+                // 128 rows are 128 / group whole tokens of one head group. Tokens past the sequence's
+                // (or, as zeros, past all) belong to rows whose results are dropped.
+                for (int h = 0; h < 2 && ok; ++h) {
+                    const int row = g.rt * kChunkRows + h * 128;
+                    if (row >= g.seq.n * p.group) break;
+                    if (queries[h] > 0) ok = __all_sync(0xffffffffu, wait(&sh.q_empty[h], (queries[h] - 1u) & 1u, kStatusHandOff));
+                    if (!ok) break;
+                    ++queries[h];
+                    if (lane == 0) {
+                        mbar_arrive_expect_tx(&sh.q_full[h], kQBytes);
+#pragma unroll
+                        for (int c = 0; c < kHalves; ++c) {
+                            load_queries_box(q_smem + h * kQBytes + c * kColumnBytes, &map_q, c * 64, g.head * p.group,
+                                             g.seq.begin + p.by_group.quotient(row), &sh.q_full[h]);
+                        }
+                    }
+                    __syncwarp();
+                }
+                if (!ok) break;
+            }
             for (int t = g.begin; t < g.end && ok; ++t) {
                 const int pos0 = (g.range.first + t) * kChunkKeys;
                 const bool partial = pos0 < g.range.lo || pos0 + kChunkKeys > g.range.hi;
-                // Lane i takes box i (and i + 32 where a tile has more than 32 boxes of a column: never, 128 / 8 = 16).
-                const int pos = pos0 + lane * box;
-                const bool mine = lane < boxes && pos < g.range.hi && pos + box > g.range.lo;
-                int page = -1, slot = 0;
-                if (mine) {
-                    const int column = page_column(view, pos);
-                    page = __ldg(view.table + g.s * view.table_stride + column);
-                    slot = pos - column * view.page_size;
+                const Box now = ahead;
+                const bool mine = now.mine;
+                const int page = now.page, slot = now.slot;
+                if (t + 1 < g.end) {
+                    ahead = find(g, t + 1);
+                } else if (more) {
+                    ahead = find(following, following.begin);
                 }
                 const int count = __popc(__ballot_sync(0xffffffffu, mine));
                 for (int which = 0; which < 2 && ok; ++which) {  // the keys, then the values
@@ -348,8 +405,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                     }
                 }
             }
-            Segment following;
-            more = plan.next(g, following);
             g = following;
         }
         if (*abort_flag) {
@@ -357,67 +412,73 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             for (uint32_t i = used > kSlots ? used - kSlots : 0; i < used; ++i) {
                 mbar_wait_bounded(&sh.kv_full[i % kSlots], (i / kSlots) & 1u, p.status, kStatusDrainTimeout);
             }
+            for (int h = 0; h < 2; ++h) {
+                if (queries[h] > 0) mbar_wait_bounded(&sh.q_full[h], (queries[h] - 1u) & 1u, p.status, kStatusDrainTimeout);
+            }
         }
-    } else if (warp == kIssueWarp) {
-        // ---------------- products ----------------
+    } else if (warp <= kIssueWarp + 1) {
+        // ---------------- products of one half ----------------
+        const int h = warp - kIssueWarp;
         constexpr uint32_t kScores = instruction<T>(kChunkKeys, false);
         constexpr uint32_t kOutput = instruction<T>(DP, true);
         const uint32_t leader = lane == 0 ? 1u : 0u;
-        uint32_t used = 0;               // slots consumed
-        uint32_t step[2] = {0u, 0u};     // tiles of each half, over all segments
-        uint32_t segments[2] = {0u, 0u};
+        const uint32_t s_at = tmem + h * 128, o_at = tmem + 256 + h * 128;
+        const uint32_t q_desc = desc_low(q_smem + h * kQBytes, 16);
+        uint32_t used = 0;      // slots consumed
+        uint32_t step = 0;      // tiles of this half, over all segments
+        uint32_t segments = 0;  // those this half works in
         bool ok = true;
         auto slot_full = [&](uint32_t i) {
             return __all_sync(0xffffffffu, wait(&sh.kv_full[i % kSlots], (i / kSlots) & 1u, kStatusTileWaitTimeout)) != 0;
         };
-        auto scores = [&](int h, uint32_t slot) {
+        auto scores = [&](uint32_t slot) {
             fence_after();
-            const uint32_t a = desc_low(q_smem + h * kQBytes, 16), b = desc_low(kv_smem + (slot % kSlots) * kSlotBytes, 16);
+            const uint32_t b = desc_low(kv_smem + (slot % kSlots) * kSlotBytes, 16);
 #pragma unroll
             for (int kk = 0; kk < DP / 16; ++kk) {
                 const uint32_t at = ((kk >> 2) * kColumnBytes + (kk & 3) * 32) >> 4;
-                mma_ss(tmem + h * 128, a + at, b + at, kScores, kk > 0, leader);
+                mma_ss(s_at, q_desc + at, b + at, kScores, kk > 0, leader);
             }
             commit_to(&sh.s_full[h], leader);
+            commit_to(&sh.kv_empty[slot % kSlots], leader);
         };
-        auto output = [&](int h, uint32_t slot, int part, bool first) {
+        auto output = [&](uint32_t slot, int part, bool first) {
             fence_after();
             const uint32_t b = desc_low(kv_smem + (slot % kSlots) * kSlotBytes, kColumnBytes);
 #pragma unroll
             for (int i = 0; i < kChunkKeys / 32; ++i) {
                 const int kk = part * (kChunkKeys / 32) + i;
-                mma_ts(tmem + 256 + h * 128, tmem + h * 128 + kk * 8, b + ((kk * 2048) >> 4), kOutput, !first || kk > 0, leader);
+                mma_ts(o_at, s_at + kk * 8, b + ((kk * 2048) >> 4), kOutput, !first || kk > 0, leader);
             }
         };
         for (bool more = true; more && ok;) {
-            const int halves = g.seq.n * p.group - g.rt * kChunkRows > 128 ? 2 : 1;
+            const bool works = h == 0 || g.seq.n * p.group - g.rt * kChunkRows > 128;
             const int tiles = g.end - g.begin;
             // Slots of this segment: keys of tile t at used + 2 t, values at used + 2 t + 1.
-            ok = slot_full(used);
-            for (int h = 0; h < halves && ok; ++h) {
-                ok = __all_sync(0xffffffffu, wait(&sh.q_full[h], segments[h] & 1u, kStatusHandOff));
-                ++segments[h];
-                if (ok) scores(h, used);
-            }
-            if (ok) commit_to(&sh.kv_empty[used % kSlots], leader);
-            for (int t = 0; t < tiles && ok; ++t) {
-                const uint32_t values = used + 2 * t + 1, keys = values + 1;
-                ok = slot_full(values);
-                for (int h = 0; h < halves && ok; ++h) {
+            if (!works) {
+                // Only hands the slots on, each once it is full (so that its phases stay in order).
+                for (int t = 0; t < 2 * tiles && ok; ++t) {
+                    ok = slot_full(used + t);
+                    if (ok && lane == 0) mbar_arrive_cta(&sh.kv_empty[(used + t) % kSlots]);
+                }
+            } else {
+                ok = slot_full(used) && __all_sync(0xffffffffu, wait(&sh.q_full[h], segments & 1u, kStatusHandOff));
+                ++segments;
+                if (ok) scores(used);
+                if (ok && tiles == 1) commit_to(&sh.q_empty[h], leader);
+                for (int t = 0; t < tiles && ok; ++t, ++step) {
+                    const uint32_t values = used + 2 * t + 1;
+                    ok = slot_full(values);
+                    if (ok && t + 1 < tiles) ok = slot_full(values + 1);  // before the weights, whose arrival is waited for
                     for (int part = 0; part < 2 && ok; ++part) {
-                        ok = __all_sync(0xffffffffu, wait(&sh.p_full[h][part], step[h] & 1u, kStatusHandOff));
-                        if (ok) output(h, values, part, t == 0);
+                        ok = __all_sync(0xffffffffu, wait(&sh.p_full[h][part], step & 1u, kStatusHandOff));
+                        if (ok) output(values, part, t == 0);
                     }
-                    ++step[h];
                     if (!ok) break;
                     commit_to(&sh.o_full[h], leader);
-                    if (h == halves - 1) commit_to(&sh.kv_empty[values % kSlots], leader);
-                    if (t + 1 < tiles) {
-                        if (h == 0) ok = slot_full(keys);
-                        if (!ok) break;
-                        scores(h, keys);
-                        if (h == halves - 1) commit_to(&sh.kv_empty[keys % kSlots], leader);
-                    }
+                    commit_to(&sh.kv_empty[values % kSlots], leader);
+                    if (t + 1 < tiles) scores(values + 1);
+                    if (t + 2 == tiles) commit_to(&sh.q_empty[h], leader);
                 }
             }
             used += 2 * tiles;
@@ -426,8 +487,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             g = following;
         }
         // No product is in flight when tensor memory is freed.
-        commit_to(&sh.drain, leader);
-        mbar_wait_bounded(&sh.drain, 0u, p.status, kStatusDrainTimeout);
+        commit_to(&sh.drain[h], leader);
+        mbar_wait_bounded(&sh.drain[h], 0u, p.status, kStatusDrainTimeout);
     }
     } else {
         // ---------------- softmax ----------------
@@ -440,8 +501,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         const float scale = p.scale_log2;
         uint32_t step = 0;  // tiles of this half, over all segments
 
-        // Brings the rows of this half of a unit to shared memory, 16 bytes per thread and row; all
-        // loads of a batch are in flight together.
+        // Brings the rows of this half of a unit to shared memory where TMA boxes do not fit them (a
+        // group that is no power of two), 16 bytes per thread and row; all loads of a batch are in
+        // flight together.
         auto load_queries = [&](const Segment& of) {
             constexpr int kPieces = DP / 8, kStep = 128 / kPieces, kBatch = 8;
             const int rows = of.seq.n * p.group - of.rt * kChunkRows - h * 128;  // live ones
@@ -464,8 +526,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                 for (int i = 0; i < kBatch; ++i) {
                     const int rr = row0 + (b + i) * kStep;
                     const uint32_t at = q_smem + h * kQBytes + (piece >> 3) * kColumnBytes + rr * 128 + (((piece & 7) ^ (rr & 7)) << 4);
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v[i].x ^ q_sign), "r"(v[i].y ^ q_sign),
-                                 "r"(v[i].z ^ q_sign), "r"(v[i].w ^ q_sign)
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v[i].x), "r"(v[i].y), "r"(v[i].z),
+                                 "r"(v[i].w)
                                  : "memory");
                 }
             }
@@ -474,7 +536,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         };
         auto half_works = [&](const Segment& of) { return h == 0 || of.seq.n * p.group - of.rt * kChunkRows > 128; };
 
-        if (half_works(g)) load_queries(g);
+        if (!q_by_tma && half_works(g)) load_queries(g);
         for (bool more = true; more;) {
             const int rows = g.seq.n * p.group - g.rt * kChunkRows;  // live rows of the unit, if below 256
             const bool works = half_works(g);
@@ -577,7 +639,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             }
             Segment following;
             more = plan.next(g, following);
-            if (ok && more) {
+            if (ok && more && !q_by_tma) {
                 // The products that read this half's queries are done (its last scores were waited
                 // for), so the next unit's scores can start while this one's output is written. A
                 // half that did not work in this unit was waited for in an earlier one.
@@ -590,70 +652,78 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             if (works && ok) {
                 fence_after();
                 const float base = top == -INFINITY ? 0.0f : top * scale;
-                const int j = p.by_group.quotient(row);
-                const long long token = g.seq.begin + j;
-                const int head = g.head * p.group + row - j * p.group;
                 const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
-                uint8_t* out = p.out + 2 * (token * p.out_token + head * p.out_head);
-                const long long at = static_cast<long long>(plan.slot(blockIdx.x, g.unit_start)) * kChunkRows + h * 128 + r;
-                float* part = p.part_o + at * DP;
-#pragma unroll 1
-                for (int c = 0; c < DP; c += 32) {
-                    float o[32];
-                    tmem_load32(o_addr + c, o);
-                    tmem_load_wait();
-                    if (!live) continue;
-                    if (whole_unit) {
-#pragma unroll
-                        for (int i = 0; i < 32; i += 8) {
-                            if (c + i < view.head_dim) {
-                                *reinterpret_cast<uint4*>(out + 2 * (c + i)) =
-                                    make_uint4(pack2<T>(o[i] * inv, o[i + 1] * inv), pack2<T>(o[i + 2] * inv, o[i + 3] * inv),
-                                               pack2<T>(o[i + 4] * inv, o[i + 5] * inv), pack2<T>(o[i + 6] * inv, o[i + 7] * inv));
-                            }
-                        }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(part + c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                if (whole_unit) {
+                    if (live && p.lse != nullptr) {
+                        const int j = p.by_group.quotient(row);
+                        p.lse[static_cast<long long>(g.seq.begin + j) * p.q_heads + g.head * p.group + row - j * p.group] =
+                            sum > 0.0f ? (base + log2f(sum)) * 0.69314718056f : (sum == 0.0f ? -INFINITY : sum);
                     }
-                }
-                if (live && whole_unit && p.lse != nullptr) {
-                    p.lse[token * p.q_heads + head] = sum > 0.0f ? (base + log2f(sum)) * 0.69314718056f : (sum == 0.0f ? -INFINITY : sum);
-                }
-                if (live && !whole_unit) {
-                    *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(top == -INFINITY ? top : base, sum);
+                    // Through shared memory, so that a store covers 64 bytes of each of 8 rows (one row
+                    // per thread would touch 32 lines with every store). Lane i writes 16 bytes of rows
+                    // i / 4 + {0, 8, 16, 24}.
+                    const uint32_t stage = stage_smem + warp * kStageBytes;
+                    const int first = h * 128 + (warp & 3) * 32;  // the warp's first row in the unit
+                    long long to[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int in_unit = first + i * 8 + (lane >> 2);
+                        const int of = g.rt * kChunkRows + in_unit;
+                        const int j = p.by_group.quotient(of);
+                        to[i] = in_unit < rows ? (g.seq.begin + j) * p.out_token + (g.head * p.group + of - j * p.group) * p.out_head : -1;
+                    }
+#pragma unroll 1
+                    for (int c = 0; c < DP; c += 32) {
+                        float o[32];
+                        tmem_load32(o_addr + c, o);
+                        tmem_load_wait();
+                        __syncwarp();
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const uint32_t at = stage + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4);
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(pack2<T>(o[8 * i] * inv, o[8 * i + 1] * inv)),
+                                         "r"(pack2<T>(o[8 * i + 2] * inv, o[8 * i + 3] * inv)),
+                                         "r"(pack2<T>(o[8 * i + 4] * inv, o[8 * i + 5] * inv)),
+                                         "r"(pack2<T>(o[8 * i + 6] * inv, o[8 * i + 7] * inv))
+                                         : "memory");
+                        }
+                        __syncwarp();
+                        const int d = c + (lane & 3) * 8;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int rr = i * 8 + (lane >> 2);
+                            uint4 v;
+                            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                         : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                                         : "r"(stage + rr * 64 + (((lane & 3) ^ ((rr >> 1) & 3)) << 4))
+                                         : "memory");
+                            if (to[i] >= 0 && d < view.head_dim) *reinterpret_cast<uint4*>(p.out + 2 * (to[i] + d)) = v;
+                        }
+                    }
+                } else {
+                    const int slot = plan.slot(blockIdx.x, g.unit_start);
+#pragma unroll 1
+                    for (int c = 0; c < DP; c += 32) {
+                        float o[32];
+                        tmem_load32(o_addr + c, o);
+                        tmem_load_wait();
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4) {
+                            *reinterpret_cast<float4*>(p.part_o + part_at<DP>(slot, (c + i) / 4, h * 128 + r)) =
+                                make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                        }
+                    }
+                    *reinterpret_cast<float2*>(p.part_ml + (static_cast<long long>(slot) * kChunkRows + h * 128 + r) * 2) =
+                        make_float2(top == -INFINITY ? top : base, sum);
+                    if (tid == 0 && g.begin == 0) {
+                        const long long last = (g.unit_start + g.range.count - 1) / plan.quota;
+                        joins[blockIdx.x] = {g.seq.begin, g.seq.n, g.rt, g.head, slot, static_cast<int>(last - blockIdx.x) + 1};
+                    }
                 }
                 fence_before();  // O is read before the next unit's products overwrite it (after this thread's next arrival)
             }
-            if (!whole_unit) {
-                __threadfence();
-                ok = softmax_barrier(ok);
-                if (ok) {
-                    if (tid == 0) {
-                        const long long c_first = g.unit_start / plan.quota, c_last = (g.unit_start + g.range.count - 1) / plan.quota;
-                        sh.last = arrive_last(p.tickets + c_first, p.epoch, static_cast<uint32_t>(c_last - c_first + 1)) ? 1 : 0;
-                    }
-                    softmax_barrier(true);
-                    if (sh.last) {
-                        __threadfence();
-                        join_partials<T, kChunkRows, DP, kSoftmaxThreads>(p, plan, g);
-                    }
-                    softmax_barrier(true);  // sh.last is read before it is written again
-                }
-            }
             if (!ok) {
                 *abort_flag = 1;
-                // The other softmax warps meet at the next cut unit's barrier: end it for them too.
-                bool met = !whole_unit;
-                while (!met && more) {
-                    g = following;
-                    met = g.begin != 0 || g.end != g.range.count;
-                    if (met) {
-                        softmax_barrier(false);
-                    } else {
-                        more = plan.next(g, following);
-                    }
-                }
                 break;
             }
             g = following;
@@ -666,6 +736,61 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     if (warp == kIssueWarp) {
         __syncwarp();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+// Joins the cut units of the chunk kernel before it, in the order of the CTAs: block (c, b) takes
+// rows 32 b .. + 31 of the unit that CTA c began. Launched behind the chunk kernel, so that all SMs
+// share the work: joined by the CTA that ended last, one unit's 256 rows took 30 us of one SM.
+constexpr int kJoinThreads = 256;
+constexpr int kJoinRows = 32;
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttnParams p, const Join* joins) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const Join join = joins[blockIdx.x];
+    const int r = blockIdx.y * kJoinRows + (threadIdx.x & 31);  // of the unit
+    const int row = join.rt * kChunkRows + r;                   // of the sequence
+    if (join.parts == 0 || row >= join.n * p.group) return;
+    constexpr int kPer = DP / 4 / (kJoinThreads / 32);  // 4-element columns per thread
+    const int column = threadIdx.x >> 5;
+    const auto slot = [&](int c) { return c == 0 ? join.first_slot : 2 * (static_cast<int>(blockIdx.x) + c); };
+    float base = -INFINITY;
+    for (int c = 0; c < join.parts; ++c) base = fmaxf(base, p.part_ml[(static_cast<long long>(slot(c)) * kChunkRows + r) * 2]);
+    if (base == -INFINITY) base = 0.0f;
+    float sum = 0.0f;
+    float4 o[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+    for (int c = 0; c < join.parts; ++c) {
+        const int s = slot(c);
+        const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (static_cast<long long>(s) * kChunkRows + r) * 2);
+        const float w = exp2f(ml.x - base);
+        sum += w * ml.y;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const float4 v = *reinterpret_cast<const float4*>(p.part_o + part_at<DP>(s, column + i * (kJoinThreads / 32), r));
+            o[i].x += w * v.x;
+            o[i].y += w * v.y;
+            o[i].z += w * v.z;
+            o[i].w += w * v.w;
+        }
+    }
+    const int j = p.by_group.quotient(row);
+    const long long token = join.begin + j;
+    const int head = join.head * p.group + row - j * p.group;
+    const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int d = (column + i * (kJoinThreads / 32)) * 4;
+        if (d < p.view.head_dim) {
+            *reinterpret_cast<uint2*>(p.out + 2 * (token * p.out_token + head * p.out_head + d)) =
+                make_uint2(pack2<T>(o[i].x * inv, o[i].y * inv), pack2<T>(o[i].z * inv, o[i].w * inv));
+        }
+    }
+    if (column == 0 && p.lse != nullptr) {
+        p.lse[token * p.q_heads + head] = sum > 0.0f ? (base + log2f(sum)) * 0.69314718056f : (sum == 0.0f ? -INFINITY : sum);
     }
 }
 
