@@ -8,11 +8,10 @@
 //     most 128; 128-byte swizzle). Pages out of range read as zeros. Where a value tile is only
 //     partly inside the unit's keys, it clears the other rows itself before it hands the tile
 //     over: a weight of 0 times a NaN left in an unused slot would be a NaN.
-//   * Warps 9 and 10 issue the products of half 0 and 1: S_h = Q_h K^T (both operands K-major in
-//     shared memory) and O_h += P_h V (P from tensor memory, V as it lies, MN-major). While the
-//     tensor cores work for one half, the softmax of the other runs. A warp of its own for each
-//     half, as the tensor cores queue only about two instructions: a warp that waits for one
-//     half's weights would hold up the other's products.
+//   * Warp 9 issues the products: S_h = Q_h K^T (both operands K-major in shared memory) and
+//     O_h += P_h V (P from tensor memory, V as it lies, MN-major), h = 0, 1 in turn. While the
+//     tensor cores work for one half, the softmax of the other runs. (Issued by a warp per half at
+//     will, the halves fell into step, all products and then all softmax: 4,700 cycles a tile.)
 //   * Warps 0-3 and 4-7 (softmax of half 0 and 1; a thread holds a row) read a row's 128 scores
 //     from tensor memory, keep the running maximum and sum, and write the weights back over the
 //     scores in the values' type. The reference point of the exponentials is moved (and O
@@ -39,9 +38,9 @@ namespace paged {
 
 constexpr int kChunkRows = 256;
 constexpr int kChunkKeys = 128;
-constexpr int kChunkThreads = 384;  // warp 11 only completes the third warpgroup
+constexpr int kChunkThreads = 384;  // warps 10 and 11 only complete the third warpgroup
 constexpr int kProducerWarp = 8;
-constexpr int kIssueWarp = 9;  // and 10
+constexpr int kIssueWarp = 9;
 // Registers: the launch gives 168 to each of 384 threads (64,512); the softmax warpgroups hold a
 // row's 128 scores and take 208, the third gives up the difference: 256 * 208 + 128 * 88 = 64,512.
 constexpr int kSoftmaxRegisters = 208;
@@ -69,15 +68,16 @@ enum : uint32_t { kStatusHandOff = 4u };  // ZCGVS_DEVICE_TMEM_WAIT_TIMEOUT
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// The issuing warp runs converged and its instructions carry the leader's predicate: operands then
-// stay in uniform registers, and a product costs a few issue slots instead of about a hundred
-// cycles (measured: 1,630 cycles for 16 products behind a one-thread branch).
-__device__ __forceinline__ void commit_to(u64* bar, uint32_t leader) {
-    asm volatile(
-        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
-        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(smem_u32(bar)),
-        "r"(leader)
-        : "memory");
+// One lane of a converged warp, chosen by the hardware: the compiler then keeps the operands of the
+// instructions behind it in uniform registers.
+__device__ __forceinline__ bool elected() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(r));
+    return r != 0u;
+}
+
+__device__ __forceinline__ void commit_to(u64* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
 // Shared-memory descriptors, 128-byte swizzle: rows of 128 bytes in groups of 8 (1024 bytes). The
@@ -95,19 +95,19 @@ __device__ __forceinline__ constexpr uint32_t instruction(int n, bool b_mn_major
            (static_cast<uint32_t>(128 >> 4) << 24);
 }
 
-__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool accumulate, uint32_t leader) {
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-        "mov.b64 da, {%1, %6};\n\tmov.b64 db, {%2, %6};\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}\n" ::"r"(d),
-        "r"(a), "r"(b), "r"(idesc), "r"(accumulate ? 1u : 0u), "r"(leader), "r"(kDescHigh));
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}\n" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(accumulate ? 1u : 0u), "r"(kDescHigh));
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool accumulate, uint32_t leader) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p, q;\n\t.reg .b64 db;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-        "mov.b64 db, {%2, %6};\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}\n" ::"r"(d),
-        "r"(a), "r"(b), "r"(idesc), "r"(accumulate ? 1u : 0u), "r"(leader), "r"(kDescHigh));
+        "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "mov.b64 db, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}\n" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(accumulate ? 1u : 0u), "r"(kDescHigh));
 }
 
 __device__ __forceinline__ void tmem_load32(uint32_t addr, float* v) {
@@ -214,7 +214,7 @@ struct ChunkShared {
     u64 raw;  // a value tile that the producer still has to clear rows of
     u64 q_full[2], q_empty[2], s_full[2], o_full[2];
     u64 p_full[2][2];  // of each half, the weights of the tile's first and second 64 keys
-    u64 drain[2];
+    u64 drain;
     uint32_t tmem;
     int abort;
 };
@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         joins[blockIdx.x].parts = 0;
         for (int s = 0; s < kSlots; ++s) {
             mbar_init(&sh.kv_full[s], 1);
-            mbar_init(&sh.kv_empty[s], 2);  // both issuing warps
+            mbar_init(&sh.kv_empty[s], 1);
         }
         mbar_init(&sh.raw, 1);
         for (int h = 0; h < 2; ++h) {
@@ -276,8 +276,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             mbar_init(&sh.p_full[h][1], 128);
             mbar_init(&sh.o_full[h], 1);
         }
-        mbar_init(&sh.drain[0], 1);
-        mbar_init(&sh.drain[1], 1);
+        mbar_init(&sh.drain, 1);
         fence_mbarrier_init();
         sh.abort = 0;
     }
@@ -416,69 +415,76 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                 if (queries[h] > 0) mbar_wait_bounded(&sh.q_full[h], (queries[h] - 1u) & 1u, p.status, kStatusDrainTimeout);
             }
         }
-    } else if (warp <= kIssueWarp + 1) {
-        // ---------------- products of one half ----------------
-        const int h = warp - kIssueWarp;
+    } else if (warp == kIssueWarp) {
+        // ---------------- products ----------------
         constexpr uint32_t kScores = instruction<T>(kChunkKeys, false);
         constexpr uint32_t kOutput = instruction<T>(DP, true);
-        const uint32_t leader = lane == 0 ? 1u : 0u;
-        const uint32_t s_at = tmem + h * 128, o_at = tmem + 256 + h * 128;
-        const uint32_t q_desc = desc_low(q_smem + h * kQBytes, 16);
-        uint32_t used = 0;      // slots consumed
-        uint32_t step = 0;      // tiles of this half, over all segments
-        uint32_t segments = 0;  // those this half works in
+        // Whatever an instruction's operands are made of comes from lane 0, so that the compiler knows
+        // them to be the same in all lanes.
+        const uint32_t tmem0 = __shfl_sync(0xffffffffu, tmem, 0);
+        uint32_t used = 0;                // slots consumed
+        uint32_t step[2] = {0u, 0u};      // tiles of each half, over all segments
+        uint32_t segments[2] = {0u, 0u};  // those each half works in
         bool ok = true;
-        auto slot_full = [&](uint32_t i) {
-            return __all_sync(0xffffffffu, wait(&sh.kv_full[i % kSlots], (i / kSlots) & 1u, kStatusTileWaitTimeout)) != 0;
-        };
-        auto scores = [&](uint32_t slot) {
+        auto all_wait = [&](u64* bar, uint32_t parity, uint32_t flag) { return __all_sync(0xffffffffu, wait(bar, parity, flag)) != 0; };
+        auto slot_full = [&](uint32_t i) { return all_wait(&sh.kv_full[i % kSlots], (i / kSlots) & 1u, kStatusTileWaitTimeout); };
+        auto scores = [&](int h, uint32_t slot, bool last_half, bool last) {
             fence_after();
-            const uint32_t b = desc_low(kv_smem + (slot % kSlots) * kSlotBytes, 16);
+            const uint32_t a = desc_low(q_smem + h * kQBytes, 16), b = desc_low(kv_smem + (slot % kSlots) * kSlotBytes, 16);
+            if (elected()) {
 #pragma unroll
-            for (int kk = 0; kk < DP / 16; ++kk) {
-                const uint32_t at = ((kk >> 2) * kColumnBytes + (kk & 3) * 32) >> 4;
-                mma_ss(s_at, q_desc + at, b + at, kScores, kk > 0, leader);
+                for (int kk = 0; kk < DP / 16; ++kk) {
+                    const uint32_t at = ((kk >> 2) * kColumnBytes + (kk & 3) * 32) >> 4;
+                    mma_ss(tmem0 + h * 128, a + at, b + at, kScores, kk > 0);
+                }
+                commit_to(&sh.s_full[h]);
+                if (last_half) commit_to(&sh.kv_empty[slot % kSlots]);
+                if (last) commit_to(&sh.q_empty[h]);
             }
-            commit_to(&sh.s_full[h], leader);
-            commit_to(&sh.kv_empty[slot % kSlots], leader);
+            __syncwarp();
         };
-        auto output = [&](uint32_t slot, int part, bool first) {
+        auto output = [&](int h, uint32_t slot, int part, bool first, bool last_half) {
             fence_after();
             const uint32_t b = desc_low(kv_smem + (slot % kSlots) * kSlotBytes, kColumnBytes);
+            if (elected()) {
 #pragma unroll
-            for (int i = 0; i < kChunkKeys / 32; ++i) {
-                const int kk = part * (kChunkKeys / 32) + i;
-                mma_ts(o_at, s_at + kk * 8, b + ((kk * 2048) >> 4), kOutput, !first || kk > 0, leader);
+                for (int i = 0; i < kChunkKeys / 32; ++i) {
+                    const int kk = part * (kChunkKeys / 32) + i;
+                    mma_ts(tmem0 + 256 + h * 128, tmem0 + h * 128 + kk * 8, b + ((kk * 2048) >> 4), kOutput, !first || kk > 0);
+                }
+                if (part == 1) {
+                    commit_to(&sh.o_full[h]);
+                    if (last_half) commit_to(&sh.kv_empty[slot % kSlots]);
+                }
             }
+            __syncwarp();
         };
         for (bool more = true; more && ok;) {
-            const bool works = h == 0 || g.seq.n * p.group - g.rt * kChunkRows > 128;
-            const int tiles = g.end - g.begin;
+            const int halves = __shfl_sync(0xffffffffu, g.seq.n * p.group - g.rt * kChunkRows > 128 ? 2 : 1, 0);
+            const int tiles = __shfl_sync(0xffffffffu, g.end - g.begin, 0);
             // Slots of this segment: keys of tile t at used + 2 t, values at used + 2 t + 1.
-            if (!works) {
-                // Only hands the slots on, each once it is full (so that its phases stay in order).
-                for (int t = 0; t < 2 * tiles && ok; ++t) {
-                    ok = slot_full(used + t);
-                    if (ok && lane == 0) mbar_arrive_cta(&sh.kv_empty[(used + t) % kSlots]);
-                }
-            } else {
-                ok = slot_full(used) && __all_sync(0xffffffffu, wait(&sh.q_full[h], segments & 1u, kStatusHandOff));
-                ++segments;
-                if (ok) scores(used);
-                if (ok && tiles == 1) commit_to(&sh.q_empty[h], leader);
-                for (int t = 0; t < tiles && ok; ++t, ++step) {
-                    const uint32_t values = used + 2 * t + 1;
-                    ok = slot_full(values);
-                    if (ok && t + 1 < tiles) ok = slot_full(values + 1);  // before the weights, whose arrival is waited for
-                    for (int part = 0; part < 2 && ok; ++part) {
-                        ok = __all_sync(0xffffffffu, wait(&sh.p_full[h][part], step & 1u, kStatusHandOff));
-                        if (ok) output(values, part, t == 0);
+            ok = slot_full(used);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if (h >= halves || !ok) break;
+                ok = all_wait(&sh.q_full[h], segments[h] & 1u, kStatusHandOff);
+                ++segments[h];
+                if (ok) scores(h, used, h == halves - 1, tiles == 1);
+            }
+            for (int t = 0; t < tiles && ok; ++t) {
+                const uint32_t values = used + 2 * t + 1;
+                ok = slot_full(values);
+                if (ok && t + 1 < tiles) ok = slot_full(values + 1);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if (h >= halves || !ok) break;
+#pragma unroll
+                    for (int part = 0; part < 2; ++part) {
+                        ok = ok && all_wait(&sh.p_full[h][part], step[h] & 1u, kStatusHandOff);
+                        if (ok) output(h, values, part, t == 0, h == halves - 1);
                     }
-                    if (!ok) break;
-                    commit_to(&sh.o_full[h], leader);
-                    commit_to(&sh.kv_empty[values % kSlots], leader);
-                    if (t + 1 < tiles) scores(values + 1);
-                    if (t + 2 == tiles) commit_to(&sh.q_empty[h], leader);
+                    ++step[h];
+                    if (ok && t + 1 < tiles) scores(h, values + 1, h == halves - 1, t + 2 == tiles);
                 }
             }
             used += 2 * tiles;
@@ -487,8 +493,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             g = following;
         }
         // No product is in flight when tensor memory is freed.
-        commit_to(&sh.drain[h], leader);
-        mbar_wait_bounded(&sh.drain[h], 0u, p.status, kStatusDrainTimeout);
+        if (elected()) commit_to(&sh.drain);
+        __syncwarp();
+        mbar_wait_bounded(&sh.drain, 0u, p.status, kStatusDrainTimeout);
     }
     } else {
         // ---------------- softmax ----------------
