@@ -18,6 +18,8 @@
 //     rescaled, in tensor memory) only when the maximum rose by more than 8 in log2 units, so
 //     weights stay below 2^8 and rescaling is rare; the result is the same, since sum and O share
 //     the reference point.
+//   * Warps 12-15 write a finished unit's O while the softmax warps are at the next unit (done by
+//     the softmax warps, a unit cost about 4 us more).
 // Tensor memory: S_0, S_1 (P over them) and O_0, O_1, 128 columns each.
 //
 // Scores, maxima, sums and O are fp32. The weights are rounded to the cache's type, as the second
@@ -38,14 +40,15 @@ namespace paged {
 
 constexpr int kChunkRows = 256;
 constexpr int kChunkKeys = 128;
-constexpr int kChunkThreads = 384;  // warps 10 and 11 only complete the third warpgroup
+constexpr int kChunkExtra = 3;  // a unit's first loads and its end, in tiles
+constexpr int kChunkThreads = 512;  // warps 10 and 11 only complete their warpgroup
 constexpr int kProducerWarp = 8;
 constexpr int kIssueWarp = 9;
-// Registers: the launch gives 168 to each of 384 threads (64,512); the softmax warpgroups hold a
-// row's 128 scores and take 208, the third gives up the difference: 256 * 208 + 128 * 88 = 64,512.
-constexpr int kSoftmaxRegisters = 208;
-constexpr int kOtherRegisters = 88;
-constexpr int kFmaOf8 = 2;  // of 8 pairs of weights, those computed by exp2_fma
+constexpr int kOutputWarp = 12;  // to 15
+// Registers: the launch gives 128 to each of 512 threads (65,536); the softmax warpgroups hold a
+// row's 128 scores and take 192, the other two give up the difference: 256 * 192 + 256 * 64 = 65,536.
+constexpr int kSoftmaxRegisters = 192;
+constexpr int kOtherRegisters = 64;
 constexpr float kRescaleAbove = 8.0f;  // log2 units
 
 template <int DP>
@@ -56,11 +59,11 @@ template <int DP>
 constexpr int chunk_slot_bytes() {
     return kChunkKeys * DP * 2;
 }
-constexpr int kStageBytes = 32 * 64;  // a softmax warp's output on its way out: 32 rows of 32 elements
+constexpr int kStageBytes = 32 * 64;  // an output warp's rows on their way out: 32 of 32 elements
 
 template <int DP>
 constexpr int chunk_smem_bytes() {
-    return kChunkRows * DP * 2 + chunk_slots<DP>() * chunk_slot_bytes<DP>() + 8 * kStageBytes + 1024;
+    return kChunkRows * DP * 2 + chunk_slots<DP>() * chunk_slot_bytes<DP>() + 4 * kStageBytes + 1024;
 }
 
 enum : uint32_t { kStatusHandOff = 4u };  // ZCGVS_DEVICE_TMEM_WAIT_TIMEOUT
@@ -187,23 +190,6 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 }
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 
-// 2^x on the FMA units, for x <= 127 (below -126 as -126): x = n + f with n the nearest integer
-// (left in the low bits by adding 1.5 * 2^23) and a polynomial of degree 4 for 2^f on [-1/2, 1/2],
-// the minimax one of the relative error (own Remez exchange: 2.6e-6 at most, 1.4e-8 on average),
-// whose exponent n is added to. The special-function unit gives 16 results per cycle and SM, and
-// 128 x 128 of them take as long as both products of a tile; a part of them goes here instead.
-__device__ __forceinline__ float2 exp2_fma(float2 x) {
-    x = make_float2(fmaxf(x.x, -126.0f), fmaxf(x.y, -126.0f));
-    const float2 n = add2(x, both(12582912.0f));
-    const float2 f = add2(x, fma2(add2(n, both(-12582912.0f)), both(-1.0f), both(0.0f)));
-    float2 y = fma2(both(0.009570102207362652f), f, both(0.05591785907745361f));
-    y = fma2(y, f, both(0.240247443318367f));
-    y = fma2(y, f, both(0.6931217908859253f));
-    y = fma2(y, f, both(0.9999992847442627f));
-    return make_float2(__int_as_float(__float_as_int(y.x) + (__float_as_int(n.x) << 23)),
-                       __int_as_float(__float_as_int(y.y) + (__float_as_int(n.y) << 23)));
-}
-
 // Called by all warps of a warpgroup, first thing in its branch: a split before the branch would
 // bound both sides by the smaller number.
 __device__ __forceinline__ void give_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegisters)); }
@@ -214,6 +200,8 @@ struct ChunkShared {
     u64 raw;  // a value tile that the producer still has to clear rows of
     u64 q_full[2], q_empty[2], s_full[2], o_full[2];
     u64 p_full[2][2];  // of each half, the weights of the tile's first and second 64 keys
+    u64 stats_full[2], o_free[2];  // a unit's row statistics are there; O and they have been read
+    float2 stats[2][128];          // reference point (log2 units) and sum of a row
     u64 drain;
     uint32_t tmem;
     int abort;
@@ -255,7 +243,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const View& view = p.view;
 
-    Planner<kChunkRows, kChunkKeys, kChunkThreads, 32> plan(p, plan_shared);
+    Planner<kChunkRows, kChunkKeys, kChunkThreads, 32, kChunkExtra> plan(p, plan_shared);
     if (!plan.start(4)) {
         if (tid == 0) joins[blockIdx.x].parts = 0;
         return;
@@ -275,6 +263,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             mbar_init(&sh.p_full[h][0], 128);
             mbar_init(&sh.p_full[h][1], 128);
             mbar_init(&sh.o_full[h], 1);
+            mbar_init(&sh.stats_full[h], 128);
+            mbar_init(&sh.o_free[h], 128);
         }
         mbar_init(&sh.drain, 1);
         fence_mbarrier_init();
@@ -301,7 +291,105 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         return true;
     };
 
-    if (warp >= kProducerWarp) {
+    if (warp >= kOutputWarp) {
+        // ---------------- output ----------------
+        give_registers();
+        const int r = tid & 127;  // row of a half = TMEM lane
+        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const uint32_t stage = stage_smem + (warp & 3) * kStageBytes;
+        uint32_t step[2] = {0u, 0u};      // tiles of each half, over all segments
+        uint32_t segments[2] = {0u, 0u};  // those each half works in
+        bool ok = true;
+        for (bool more = true; more && ok;) {
+            const int rows = g.seq.n * p.group - g.rt * kChunkRows;  // live rows of the unit, if below 256
+            const bool whole_unit = g.begin == 0 && g.end == g.range.count;
+            const int slot = plan.slot(blockIdx.x, g.unit_start);
+            if (tid == kOutputWarp * 32 && !whole_unit && g.begin == 0) {
+                const long long last = (g.unit_start + g.range.count - 1) / plan.quota;
+                joins[blockIdx.x] = {g.seq.begin, g.seq.n, g.rt, g.head, slot, static_cast<int>(last - blockIdx.x) + 1};
+            }
+            for (int h = 0; h < 2 && ok; ++h) {
+                if (h * 128 >= rows) break;
+                step[h] += g.end - g.begin;
+                // Through shared memory, so that a store covers 64 bytes of each of 8 rows (one row
+                // per thread would touch 32 lines with every store). Lane i writes 16 bytes of rows
+                // i / 4 + {0, 8, 16, 24} of the warp's.
+                const int first = h * 128 + (warp & 3) * 32;  // the warp's first row in the unit
+                long long to[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int in_unit = first + i * 8 + (lane >> 2);
+                    const int of = g.rt * kChunkRows + in_unit;
+                    const int j = p.by_group.quotient(of);
+                    to[i] = in_unit < rows ? (g.seq.begin + j) * p.out_token + (g.head * p.group + of - j * p.group) * p.out_head : -1;
+                }
+                ok = wait(&sh.stats_full[h], segments[h] & 1u, kStatusHandOff) && wait(&sh.o_full[h], (step[h] - 1u) & 1u, kStatusHandOff);
+                ++segments[h];
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                fence_after();
+                const float2 stats = sh.stats[h][r];
+                const float sum = stats.y;
+                const uint32_t o_addr = tmem + lanes + 256 + h * 128;
+                if (whole_unit) {
+                    const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
+                    if (h * 128 + r < rows && p.lse != nullptr) {
+                        const int row = g.rt * kChunkRows + h * 128 + r;
+                        const int j = p.by_group.quotient(row);
+                        p.lse[static_cast<long long>(g.seq.begin + j) * p.q_heads + g.head * p.group + row - j * p.group] =
+                            sum > 0.0f ? (stats.x + log2f(sum)) * 0.69314718056f : (sum == 0.0f ? -INFINITY : sum);
+                    }
+#pragma unroll 1
+                    for (int c = 0; c < DP; c += 32) {
+                        float o[32];
+                        tmem_load32(o_addr + c, o);
+                        tmem_load_wait();
+                        __syncwarp();
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const uint32_t at = stage + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4);
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(pack2<T>(o[8 * i] * inv, o[8 * i + 1] * inv)),
+                                         "r"(pack2<T>(o[8 * i + 2] * inv, o[8 * i + 3] * inv)),
+                                         "r"(pack2<T>(o[8 * i + 4] * inv, o[8 * i + 5] * inv)),
+                                         "r"(pack2<T>(o[8 * i + 6] * inv, o[8 * i + 7] * inv))
+                                         : "memory");
+                        }
+                        __syncwarp();
+                        const int d = c + (lane & 3) * 8;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int rr = i * 8 + (lane >> 2);
+                            uint4 v;
+                            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                         : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                                         : "r"(stage + rr * 64 + (((lane & 3) ^ ((rr >> 1) & 3)) << 4))
+                                         : "memory");
+                            if (to[i] >= 0 && d < view.head_dim) *reinterpret_cast<uint4*>(p.out + 2 * (to[i] + d)) = v;
+                        }
+                    }
+                } else {
+#pragma unroll 1
+                    for (int c = 0; c < DP; c += 32) {
+                        float o[32];
+                        tmem_load32(o_addr + c, o);
+                        tmem_load_wait();
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4) {
+                            *reinterpret_cast<float4*>(p.part_o + part_at<DP>(slot, (c + i) / 4, h * 128 + r)) =
+                                make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                        }
+                    }
+                    *reinterpret_cast<float2*>(p.part_ml + (static_cast<long long>(slot) * kChunkRows + h * 128 + r) * 2) = stats;
+                }
+                fence_before();
+                mbar_arrive_cta(&sh.o_free[h]);
+            }
+            if (!ok) break;
+            Segment following;
+            more = plan.next(g, following);
+            g = following;
+        }
+    } else if (warp >= kProducerWarp) {
     give_registers();
     if (warp == kProducerWarp) {
         // ---------------- producer ----------------
@@ -480,6 +568,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                     if (h >= halves || !ok) break;
 #pragma unroll
                     for (int part = 0; part < 2; ++part) {
+                        if (t == 0 && part == 0 && segments[h] > 1) {  // the last unit's output has been read
+                            ok = all_wait(&sh.o_free[h], segments[h] & 1u, kStatusHandOff);
+                        }
                         ok = ok && all_wait(&sh.p_full[h][part], step[h] & 1u, kStatusHandOff);
                         if (ok) output(h, values, part, t == 0, h == halves - 1);
                     }
@@ -506,7 +597,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         const uint32_t s_addr = tmem + lanes + h * 128;
         const uint32_t o_addr = tmem + lanes + 256 + h * 128;
         const float scale = p.scale_log2;
-        uint32_t step = 0;  // tiles of this half, over all segments
+        uint32_t step = 0;      // tiles of this half, over all segments
+        uint32_t segments = 0;  // those this half works in
 
         // Brings the rows of this half of a unit to shared memory where TMA boxes do not fit them (a
         // group that is no power of two), 16 bytes per thread and row; all loads of a batch are in
@@ -547,7 +639,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         for (bool more = true; more;) {
             const int rows = g.seq.n * p.group - g.rt * kChunkRows;  // live rows of the unit, if below 256
             const bool works = half_works(g);
-            const bool whole_unit = g.begin == 0 && g.end == g.range.count;
             const int row = g.rt * kChunkRows + h * 128 + r;  // of the sequence
             const bool live = h * 128 + r < rows;
             bool ok = true;
@@ -572,10 +663,13 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                     const int pos0 = (g.range.first + t) * kChunkKeys;
                     const bool masked = pos0 < all_lo || pos0 + kChunkKeys > all_hi;
                     if (masked) {
-                        const int a = lo - pos0;
-                        const uint32_t n = static_cast<uint32_t>(max(hi - lo, 0));
+                        const auto below = [](int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; };
 #pragma unroll
-                        for (int c = 0; c < 128; ++c) s[c] = static_cast<uint32_t>(c - a) < n ? s[c] : -INFINITY;
+                        for (int w = 0; w < 128; w += 32) {
+                            const uint32_t seen = below(hi - pos0 - w) & ~below(lo - pos0 - w);
+#pragma unroll
+                            for (int c = 0; c < 32; ++c) s[w + c] = (seen >> c) & 1u ? s[w + c] : -INFINITY;
+                        }
                     }
                     float m[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
@@ -614,17 +708,13 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                     const float2 base2 = both(top == -INFINITY ? 0.0f : -top * scale), scale2 = both(scale);
                     float2 part[2] = {both(0.0f), both(0.0f)};
                     // Each half of the keys is handed over as soon as its weights are written.
-                    auto weigh = [&](auto fma_of_8, int from) {
+#pragma unroll
+                    for (int from = 0; from < 128; from += 64) {
                         uint32_t packed[32];
 #pragma unroll
                         for (int c = 0; c < 64; c += 2) {
                             const float2 x = fma2(make_float2(s[from + c], s[from + c + 1]), scale2, base2);
-                            float2 w;
-                            if ((c >> 1) % 8 < fma_of_8) {
-                                w = exp2_fma(x);
-                            } else {
-                                w = make_float2(exp2_fast(x.x), exp2_fast(x.y));
-                            }
+                            const float2 w = make_float2(exp2_fast(x.x), exp2_fast(x.y));
                             part[(c >> 1) & 1] = add2(part[(c >> 1) & 1], w);
                             packed[c >> 1] = pack2<T>(w.x, w.y);
                         }
@@ -632,13 +722,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                         tmem_store_wait();
                         fence_before();
                         mbar_arrive_cta(&sh.p_full[h][from / 64]);
-                    };
-                    if (masked) {  // exp2_fma gives no zero
-                        weigh(std::integral_constant<int, 0>{}, 0);
-                        weigh(std::integral_constant<int, 0>{}, 64);
-                    } else {
-                        weigh(std::integral_constant<int, kFmaOf8>{}, 0);
-                        weigh(std::integral_constant<int, kFmaOf8>{}, 64);
                     }
                     part[0] = add2(part[0], part[1]);
                     sum += part[0].x + part[0].y;
@@ -653,81 +736,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                 if (half_works(following)) load_queries(following);
             }
             if (works && ok) {
-                // The unit's rows, or this CTA's part of them.
-                ok = __all_sync(0xffffffffu, wait(&sh.o_full[h], (step - 1u) & 1u, kStatusHandOff));
-            }
-            if (works && ok) {
-                fence_after();
-                const float base = top == -INFINITY ? 0.0f : top * scale;
-                const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
-                if (whole_unit) {
-                    if (live && p.lse != nullptr) {
-                        const int j = p.by_group.quotient(row);
-                        p.lse[static_cast<long long>(g.seq.begin + j) * p.q_heads + g.head * p.group + row - j * p.group] =
-                            sum > 0.0f ? (base + log2f(sum)) * 0.69314718056f : (sum == 0.0f ? -INFINITY : sum);
-                    }
-                    // Through shared memory, so that a store covers 64 bytes of each of 8 rows (one row
-                    // per thread would touch 32 lines with every store). Lane i writes 16 bytes of rows
-                    // i / 4 + {0, 8, 16, 24}.
-                    const uint32_t stage = stage_smem + warp * kStageBytes;
-                    const int first = h * 128 + (warp & 3) * 32;  // the warp's first row in the unit
-                    long long to[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int in_unit = first + i * 8 + (lane >> 2);
-                        const int of = g.rt * kChunkRows + in_unit;
-                        const int j = p.by_group.quotient(of);
-                        to[i] = in_unit < rows ? (g.seq.begin + j) * p.out_token + (g.head * p.group + of - j * p.group) * p.out_head : -1;
-                    }
-#pragma unroll 1
-                    for (int c = 0; c < DP; c += 32) {
-                        float o[32];
-                        tmem_load32(o_addr + c, o);
-                        tmem_load_wait();
-                        __syncwarp();
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const uint32_t at = stage + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4);
-                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(pack2<T>(o[8 * i] * inv, o[8 * i + 1] * inv)),
-                                         "r"(pack2<T>(o[8 * i + 2] * inv, o[8 * i + 3] * inv)),
-                                         "r"(pack2<T>(o[8 * i + 4] * inv, o[8 * i + 5] * inv)),
-                                         "r"(pack2<T>(o[8 * i + 6] * inv, o[8 * i + 7] * inv))
-                                         : "memory");
-                        }
-                        __syncwarp();
-                        const int d = c + (lane & 3) * 8;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int rr = i * 8 + (lane >> 2);
-                            uint4 v;
-                            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                                         : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                                         : "r"(stage + rr * 64 + (((lane & 3) ^ ((rr >> 1) & 3)) << 4))
-                                         : "memory");
-                            if (to[i] >= 0 && d < view.head_dim) *reinterpret_cast<uint4*>(p.out + 2 * (to[i] + d)) = v;
-                        }
-                    }
-                } else {
-                    const int slot = plan.slot(blockIdx.x, g.unit_start);
-#pragma unroll 1
-                    for (int c = 0; c < DP; c += 32) {
-                        float o[32];
-                        tmem_load32(o_addr + c, o);
-                        tmem_load_wait();
-#pragma unroll
-                        for (int i = 0; i < 32; i += 4) {
-                            *reinterpret_cast<float4*>(p.part_o + part_at<DP>(slot, (c + i) / 4, h * 128 + r)) =
-                                make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-                        }
-                    }
-                    *reinterpret_cast<float2*>(p.part_ml + (static_cast<long long>(slot) * kChunkRows + h * 128 + r) * 2) =
-                        make_float2(top == -INFINITY ? top : base, sum);
-                    if (tid == 0 && g.begin == 0) {
-                        const long long last = (g.unit_start + g.range.count - 1) / plan.quota;
-                        joins[blockIdx.x] = {g.seq.begin, g.seq.n, g.rt, g.head, slot, static_cast<int>(last - blockIdx.x) + 1};
-                    }
-                }
-                fence_before();  // O is read before the next unit's products overwrite it (after this thread's next arrival)
+                if (segments > 0) ok = __all_sync(0xffffffffu, wait(&sh.o_free[h], (segments - 1u) & 1u, kStatusHandOff));
+                ++segments;
+                sh.stats[h][r] = make_float2(top == -INFINITY ? top : top * scale, sum);
+                mbar_arrive_cta(&sh.stats_full[h]);
             }
             if (!ok) {
                 *abort_flag = 1;

@@ -2,13 +2,13 @@
 //
 // The rows of a sequence are its (new token, query head of one key/value head's group) pairs,
 // token major: row r is token r / group. They are cut into row tiles of R rows; a unit is one row
-// tile of one key/value head, and its cost is the number of KT-key tiles that any of its rows
-// sees (at least 1, so that rows that see nothing are written too). All key tiles of all units,
-// in the order (sequence, row tile, head, key tile), form one line; every CTA takes the same
-// number of consecutive key tiles of it, whatever the lengths, so all end together. A unit that
-// is cut between CTAs leaves one partial result per CTA (unnormalised sums, running maximum and
-// sum), and the CTA that finishes last joins them in the order of the CTAs: no CTA waits for
-// another, and the result does not depend on which one was last.
+// tile of one key/value head. On a line lie, for every unit in the order (sequence, row tile,
+// head), EXTRA places for the time that a unit takes apart from its keys, then a place for each
+// KT-key tile that any of its rows sees (at least 1, so that rows that see nothing are written
+// too). Every CTA takes the same number of consecutive places, whatever the lengths, so all end
+// together. A unit that is cut between CTAs leaves one partial result per CTA (unnormalised sums,
+// running maximum and sum), which are joined in the order of the CTAs: no CTA waits for another,
+// and the result does not depend on which one was last.
 //
 // Every CTA computes its own part of the line from the lengths on the device (about 2 us, no
 // launch of its own): a scan over the sequences, then a warp's scan over the row tiles of the
@@ -104,7 +104,7 @@ struct Segment {
     int s, rt, head;
     UnitRange range;
     int begin, end;
-    long long unit_start;  // the unit's first key tile on the line
+    long long unit_start;  // the place of the unit's first key tile on the line
 };
 
 constexpr int kCachedSequences = 512;
@@ -121,12 +121,12 @@ struct PlanShared {
 
 // GROUP lanes add up the row tiles of one sequence: 1 where sequences have few row tiles, 32
 // where they may have hundreds.
-template <int R, int KT, int THREADS, int GROUP>
+template <int R, int KT, int THREADS, int GROUP, int EXTRA>
 struct Planner {
     const AttnParams& p;
     PlanShared<THREADS>& sh;
-    long long total = 0;  // key tiles on the line
-    long long quota = 0;  // key tiles per CTA
+    long long total = 0;  // places on the line
+    long long quota = 0;  // places per CTA
     long long at = 0, end = 0;  // this CTA's part that is left
 
     __device__ Planner(const AttnParams& params, PlanShared<THREADS>& shared) : p(params), sh(shared) {}
@@ -143,23 +143,24 @@ struct Planner {
 
     __device__ __forceinline__ int row_tiles(const Sequence& q) const { return (q.n * p.group + R - 1) / R; }
 
-    __device__ long long sequence_tiles(const Sequence& q, int lane) const {
+    // Places of a sequence (of this group's lane).
+    __device__ long long sequence_places(const Sequence& q, int lane) const {
         if (!mine(q)) return 0;
         long long sum = 0;
         const int tiles = row_tiles(q);
-        for (int rt = lane; rt < tiles; rt += GROUP) sum += unit_range<R, KT>(p, q, rt).count;
+        for (int rt = lane; rt < tiles; rt += GROUP) sum += unit_range<R, KT>(p, q, rt).count + EXTRA;
         return sum * p.view.kv_heads;
     }
 
-    // Key tiles of sequence base + threadIdx.x (0 past the last); every thread calls it.
-    __device__ long long chunk_tiles(int base) const {
+    // Places of sequence base + threadIdx.x (0 past the last); every thread calls it.
+    __device__ long long chunk_places(int base) const {
         const int tid = threadIdx.x;
         const int left = min(THREADS, p.view.sequences - base);
         if constexpr (GROUP == 1) {
-            return tid < left ? sequence_tiles(sequence(base + tid), 0) : 0;
+            return tid < left ? sequence_places(sequence(base + tid), 0) : 0;
         } else {
             for (int i = tid >> 5; i < left; i += THREADS / 32) {
-                long long c = sequence_tiles(sequence(base + i), tid & 31);
+                long long c = sequence_places(sequence(base + i), tid & 31);
                 for (int o = 16; o >= 1; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
                 if ((tid & 31) == 0) sh.count[i] = c;
             }
@@ -200,7 +201,7 @@ struct Planner {
         __syncthreads();
         long long c = 0, upto = 0, all = 0;
         for (int base = 0; base < sequences; base += THREADS) {
-            c = chunk_tiles(base);
+            c = chunk_places(base);
             upto = scan(c, all);
             total += all;
         }
@@ -211,7 +212,7 @@ struct Planner {
         long long before = 0;
         for (int base = 0; base < sequences; base += THREADS) {
             if (sequences > THREADS) {  // else the values of the only chunk are still here
-                c = chunk_tiles(base);
+                c = chunk_places(base);
                 upto = scan(c, all);
             }
             if (at >= before + upto - c && at < before + upto) {
@@ -232,7 +233,8 @@ struct Planner {
                 const int rt = base + tid;
                 UnitRange u{};
                 if (rt < tiles) u = unit_range<R, KT>(p, g.seq, rt);
-                const long long cost = static_cast<long long>(u.count) * p.view.kv_heads;
+                const int unit = u.count + EXTRA;
+                const long long cost = static_cast<long long>(unit) * p.view.kv_heads;
                 long long sum = cost;
                 for (int o = 1; o < 32; o <<= 1) {
                     const long long t = __shfl_up_sync(0xffffffffu, sum, o);
@@ -244,10 +246,11 @@ struct Planner {
                         const long long in = rest - (sum - cost);
                         g.rt = rt;
                         g.range = u;
-                        g.head = static_cast<int>(in / u.count);
-                        g.begin = static_cast<int>(in % u.count);
-                        g.end = static_cast<int>(min(static_cast<long long>(u.count), g.begin + (end - at)));
-                        g.unit_start = at - g.begin;
+                        g.head = static_cast<int>(in / unit);
+                        const int place = static_cast<int>(in % unit);  // in the unit
+                        g.unit_start = at - place + EXTRA;
+                        g.begin = max(place - EXTRA, 0);
+                        g.end = static_cast<int>(min(static_cast<long long>(u.count), end - g.unit_start));
                         sh.segment = g;
                     }
                     break;
@@ -256,14 +259,15 @@ struct Planner {
             }
         }
         __syncthreads();
-        return true;
+        // A part that ends before its unit's first key tile holds no work: the next CTA begins there.
+        return sh.segment.end > sh.segment.begin;
     }
 
     // Moves on to the CTA's next segment, after `done`. False when there is none. Only thread 0's
     // shared copy is written; callers synchronise before they read it.
     __device__ bool next(const Segment& done, Segment& g) {
-        at += done.end - done.begin;
-        if (at >= end) return false;
+        at = done.unit_start + done.end;
+        if (at + EXTRA >= end) return false;
         g = done;
         if (++g.head == p.view.kv_heads) {
             g.head = 0;
@@ -276,8 +280,8 @@ struct Planner {
             g.range = unit_range<R, KT>(p, g.seq, g.rt);
         }
         g.begin = 0;
-        g.end = static_cast<int>(min(static_cast<long long>(g.range.count), end - at));
-        g.unit_start = at;
+        g.unit_start = at + EXTRA;
+        g.end = static_cast<int>(min(static_cast<long long>(g.range.count), end - g.unit_start));
         return true;
     }
 

@@ -24,6 +24,7 @@ namespace paged {
 
 constexpr int kStreamThreads = 128;
 constexpr int kStreamKeys = 64;  // keys per tile
+constexpr int kStreamExtra = 1;  // a unit's fill and end, in tiles
 
 template <int DP>
 constexpr int stream_stage_bytes() {
@@ -103,7 +104,7 @@ __global__ void __launch_bounds__(kStreamThreads, stream_ctas_per_sm<DP>()) stre
     const View& view = p.view;
     const int d_pieces = view.head_dim / 8;
 
-    Planner<R, kStreamKeys, kStreamThreads, 1> plan(p, plan_shared);
+    Planner<R, kStreamKeys, kStreamThreads, 1, kStreamExtra> plan(p, plan_shared);
     if (!plan.start(1)) return;
     Segment g = plan_shared.segment;
 
