@@ -5,18 +5,26 @@
 // sums stay below 2^59), so every sum below is exact, whatever its order: the token does not
 // depend on the split over CTAs, and integer atomics may build histograms.
 //
-// Bound by reading the logits once. A cluster of 1 to 8 CTAs takes a row; each keeps its slice in
-// shared memory in the logits' own type, so that everything after the first pass stays on chip:
-//   1. load, maximum and minimum of the row (cluster-wide);
-//   2. where top-k or top-p cuts: a histogram of the slice over 2048 bins of the distance m - x,
-//      linear up to the distance where weights become 0 (tokens beyond weigh nothing and rank
-//      last, so they change no result); each CTA then sums its share of the bins over the cluster;
-//   3. a cut by count or by weight: the bin where the running sum reaches it, then the bin's few
-//      tokens are ranked against one another by (logit descending, id ascending). A bin of more
-//      than 1024 (equal or clustered logits) is cut into 2048 again by the tokens' 64-bit rank
-//      order, as often as needed (each time 11 bits of at most 64);
-//   4. the kept weights are summed per warp in ascending id order, and the warp that the drawn
-//      number falls into walks its tokens.
+// Bound by reading the logits once; in practice by the instructions spent per logit, so each path
+// spends few on the many tokens that cannot be drawn. A cluster of 1 to 8 CTAs takes a row; each
+// keeps its slice in shared memory in the logits' own type, so that everything after the first pass
+// stays on chip. After the row's maximum is known:
+//   * top-k up to 256: in each CTA, the q-th largest of its threads' maxima, q C >= k. The smallest
+//     of these over the cluster is a lower bound of the k-th largest logit (q distinct threads of
+//     each of C CTAs hold one at or above it), and few more than k tokens reach it. They are listed
+//     and ranked against one another, and one CTA applies all filters to the list.
+//   * otherwise, where top-k or top-p cuts: a histogram of token counts over 4096 bins of the
+//     distance m - x, linear up to the distance where weights become 0 (tokens beyond weigh nothing
+//     and rank last, so they change no result), with exact weights in the first 1024 bins (down to
+//     8e-4 of the largest weight, few tokens). A cut by count lies in one bin. A cut by weight is
+//     estimated with the bins' middle weights; one pass then sums the weights before the estimated
+//     bins exactly and lists their tokens, which are ranked against one another by (logit
+//     descending, id ascending). Should the exact sums put the cut outside these bins, or are they
+//     too full (equal or clustered logits), the bins that may hold it by the weights of all bins'
+//     edges are taken and cut again by the tokens' 64-bit rank order, with exact weights, as often
+//     as needed (8 bits of at most 64 each time).
+//   * the kept weights are summed per warp in ascending id order, and the warp that the drawn number
+//     falls into walks its tokens.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -33,8 +41,12 @@ namespace {
 
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
-constexpr int kBins = 2048;
-constexpr int kList = 1024;       // tokens of a bin that are ranked directly
+constexpr int kBins = 4096;
+constexpr int kHeavyBins = 1024;  // those with exact weights
+constexpr int kSubBins = 256;     // of bins that are cut again
+constexpr int kOwnList = 512;     // listed tokens of a CTA
+constexpr int kList = 1024;       // and of a cluster: they are ranked against one another
+constexpr int kDirect = 256;      // largest top-k that is taken from a list at once
 constexpr float kUnits = 1099511627776.0f;  // 2^40
 constexpr float kWeightless = 28.5f;        // exp(-28.5) * 2^40 rounds to 0
 constexpr int kMaxCluster = 8;
@@ -55,21 +67,31 @@ struct SampleParams {
 
 // What the CTAs of a cluster show one another.
 struct Shared {
-    float top, low;            // of the slice
-    u64 best;                  // smallest rank order value etc. (see the passes)
-    u64 weight;                // kept weight of the slice
+    float top;                 // of the slice
+    float bound;               // no top-k logit is below it
+    u64 best;                  // the slice's first ranked token
+    u64 weight[2];             // sums of weights of the slice
     unsigned chunk_count[2];   // of this CTA's share of the bins, per level
     u64 chunk_mass[2];
     unsigned listed;           // entries of this CTA's list
-    u64 range_hi, range_lo;    // rank order values of a bin's members
+    u64 range_hi, range_lo;    // rank order values of the listed bins' tokens
     // Within the CTA.
     u64 warp_u64[kWarps];
     unsigned warp_u32[kWarps];
     float warp_f32[2][kWarps];
-    int bin;
+    unsigned digit[256];
+    int bin[2];
     unsigned bin_count, before_count;
     u64 before_mass;
-    u64 cut, cut_mass;
+    u64 cut;
+    int kept;
+};
+
+// The last kept token; everything ranked at or before it is kept. x = -inf: all.
+struct Limit {
+    float x;
+    int id;
+    __device__ __forceinline__ bool keeps(float v, int i) const { return v > x || (v == x && i <= id); }
 };
 
 template <typename T>
@@ -83,8 +105,11 @@ struct Vec<float> {
         x[2] = __uint_as_float(v.z);
         x[3] = __uint_as_float(v.w);
     }
-    static __device__ __forceinline__ float load(const float* p) { return *p; }
     static __device__ __forceinline__ float lowest() { return -INFINITY; }
+    // The largest of them and x, NaN ignored.
+    static __device__ __forceinline__ float highest(const uint4& v, float x) {
+        return fmaxf(x, fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w))));
+    }
 };
 template <typename T>
 struct Vec16 {
@@ -101,13 +126,21 @@ struct Vec16 {
 };
 template <>
 struct Vec<__half> : Vec16<__half> {
-    static __device__ __forceinline__ float load(const __half* p) { return __half2float(*p); }
     static __device__ __forceinline__ __half lowest() { return __ushort_as_half(0xfc00); }
+    static __device__ __forceinline__ float highest(const uint4& v, float x) {
+        const __half2* h = reinterpret_cast<const __half2*>(&v);
+        const float2 m = __half22float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+        return fmaxf(x, fmaxf(m.x, m.y));
+    }
 };
 template <>
 struct Vec<__nv_bfloat16> : Vec16<__nv_bfloat16> {
-    static __device__ __forceinline__ float load(const __nv_bfloat16* p) { return __bfloat162float(*p); }
     static __device__ __forceinline__ __nv_bfloat16 lowest() { return __ushort_as_bfloat16(0xff80); }
+    static __device__ __forceinline__ float highest(const uint4& v, float x) {
+        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
+        const float2 m = __bfloat1622float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+        return fmaxf(x, fmaxf(m.x, m.y));
+    }
 };
 
 // Rank order value: larger is ranked earlier. 0 is below every token's.
@@ -127,67 +160,127 @@ struct Row {
     cg::cluster_group cluster;
     T* data;                 // [slice]
     unsigned* raw_count;     // [kBins]
-    u64* raw_mass;           // [kBins]
-    u64* own_list;           // [2][kList]: rank values, weights; shares memory with the histogram
+    u64* raw_mass;           // [kHeavyBins]
+    u64* own_list;           // [2][kOwnList]: rank values, weights; shares memory with the histogram
     u64* list;               // [2][kList]
-    unsigned* merged_count;  // [2][kBins / C]
-    u64* merged_mass;        // [2][kBins / C]
+    unsigned* merged_count;  // [kBins / C], then [kSubBins / C]
+    u64* merged_mass;        // [kHeavyBins / C], then [kSubBins / C]
     int ranks, rank, first;  // CTAs of the cluster, this one, its slice's first token
     int tid, lane, warp;
-    float top, t, spread, to_bin;
-    bool need_mass;
+    float top, t, per_t, spread, to_bin;
 
     __device__ Row(const SampleParams& params, Shared& shared) : p(params), sh(shared), cluster(cg::this_cluster()) {}
 
-    // Calls f(x, id) for every token of the slice that can be drawn; ids ascend within a warp's
-    // share, which is contiguous.
+    // Calls f(x, id) for every token of the slice that can be drawn (not -inf, not NaN); ids ascend
+    // within a warp's share, which is contiguous.
     template <typename F>
     __device__ __forceinline__ void each(F f) const {
         const int share = p.slice / kWarps;
+#pragma unroll 2
         for (int at = warp * share + lane * V::kN; at < (warp + 1) * share; at += 32 * V::kN) {
             float x[V::kN];
             V::unpack(*reinterpret_cast<const uint4*>(data + at), x);
 #pragma unroll
             for (int i = 0; i < V::kN; ++i) {
-                if (x[i] != -INFINITY) f(x[i], first + at + i);
+                if (x[i] > -INFINITY) f(x[i], first + at + i);
+            }
+        }
+    }
+
+    // Calls f(x, id) for the tokens at or above `least` (> -inf); whole vectors below it cost one test.
+    template <typename F>
+    __device__ __forceinline__ void each_from(float least, F f) const {
+        const int share = p.slice / kWarps;
+#pragma unroll 2
+        for (int at = warp * share + lane * V::kN; at < (warp + 1) * share; at += 32 * V::kN) {
+            const uint4 v = *reinterpret_cast<const uint4*>(data + at);
+            if (!(V::highest(v, -INFINITY) >= least)) continue;
+            float x[V::kN];
+            V::unpack(v, x);
+#pragma unroll
+            for (int i = 0; i < V::kN; ++i) {
+                if (x[i] >= least) f(x[i], first + at + i);
             }
         }
     }
 
     __device__ __forceinline__ float distance(float x) const { return x == top ? 0.0f : top - x; }
-    __device__ __forceinline__ float share_of(float x) const { return x == top ? 1.0f : expf(__fdiv_rn(x - top, t)); }
+    // exp((x - m) / t), rounded as the function's value at the correctly rounded quotient. With the
+    // correctly rounded reciprocal y of t, Markstein's iteration q' = q + (a - t q) y gives the
+    // correctly rounded quotient from one that is within a unit of the last place (two steps, from
+    // a y). Quotients so small that the remainder underflows have the exponential 1 either way.
+    // (fmaxf: 0 where both the largest logit and the temperature are infinite.)
+    __device__ __forceinline__ float share_of(float x) const {
+        if (per_t == 0.0f) return x == top ? 1.0f : fmaxf(expf(__fdiv_rn(x - top, t)), 0.0f);
+        const float a = x - top;
+        float q = a * per_t;
+        q = fmaf(fmaf(-t, q, a), per_t, q);
+        q = fmaf(fmaf(-t, q, a), per_t, q);
+        return expf(q);
+    }
     __device__ __forceinline__ u64 weight(float x) const { return static_cast<u64>(__float2ll_rn(share_of(x) * kUnits)); }
-    __device__ __forceinline__ int bin_of(float d) const { return min(kBins - 1, static_cast<int>(d * to_bin)); }
+    // Adds rint(2^40 e) to hi * 2^20 + lo: e 2^20 = h + l with h the nearest integer (both exact), and
+    // rint(2^40 e) = 2^20 h + rint(2^20 l). Integers come out of the low bits after adding 1.5 * 2^23.
+    __device__ __forceinline__ static void add_units(float e, int& hi, int& lo) {
+        const float big = 12582912.0f, unit = 1048576.0f;
+        const float h = fmaf(e, unit, big);
+        const float l = fmaf(fmaf(e, unit, big - h), unit, big);
+        hi += __float_as_int(h) - 0x4B400000;
+        lo += __float_as_int(l) - 0x4B400000;
+    }
+    __device__ __forceinline__ static u64 units(int hi, int lo) {
+        return static_cast<u64>((static_cast<long long>(hi) << 20) + lo);
+    }
+    // The bin of a distance at most `spread`: the nearest integer of d * to_bin.
+    __device__ __forceinline__ int bin_of(float d) const {
+        return min(kBins - 1, __float_as_int(fmaf(d, to_bin, 8388608.0f)) & 0x7FFFFF);
+    }
 
-    __device__ void clear_histogram() {
-        for (int b = tid; b < kBins; b += kThreads) {
-            raw_count[b] = 0u;
-            raw_mass[b] = 0ull;
-        }
+    // Level 0: the distances. Level 1: some of its bins cut again.
+    __device__ __forceinline__ static int bins_of(int level) { return level == 0 ? kBins : kSubBins; }
+    __device__ __forceinline__ static int masses_of(int level) { return level == 0 ? kHeavyBins : kSubBins; }
+    __device__ void clear_histogram(int level) {
+        for (int b = tid; b < bins_of(level); b += kThreads) raw_count[b] = 0u;
+        for (int b = tid; b < masses_of(level); b += kThreads) raw_mass[b] = 0ull;
         __syncthreads();
     }
 
-    __device__ __forceinline__ void count(int b, float x) {
-        atomicAdd(raw_count + b, 1u);
-        if (need_mass) atomicAdd(raw_mass + b, weight(x));
+    // Sum of v over the cluster, for all its threads. `which`: two sums may follow one another
+    // without a barrier between them.
+    __device__ u64 cluster_sum(u64 v, int which) {
+        v = warp_sum_u64(v);
+        __syncthreads();
+        if (lane == 0) sh.warp_u64[warp] = v;
+        __syncthreads();
+        if (tid == 0) {
+            u64 all = 0ull;
+            for (int w = 0; w < kWarps; ++w) all += sh.warp_u64[w];
+            sh.weight[which] = all;
+        }
+        cluster.sync();
+        u64 all = 0ull;
+        for (int r = 0; r < ranks; ++r) all += cluster.map_shared_rank(&sh, r)->weight[which];
+        return all;
     }
 
     // Sums this CTA's share of the bins over the cluster.
     __device__ void merge(int level) {
         cluster.sync();
-        const int n = kBins / ranks;
+        const int n = bins_of(level) / ranks, heavy = masses_of(level) / ranks;
+        unsigned* counts = merged_count + (level == 0 ? 0 : kBins / ranks);
+        u64* masses = merged_mass + (level == 0 ? 0 : kHeavyBins / ranks);
         unsigned c_all = 0;
         u64 m_all = 0;
         for (int b = tid; b < n; b += kThreads) {
             unsigned c = 0;
-            u64 m = 0;
-            for (int r = 0; r < ranks; ++r) {
-                c += cluster.map_shared_rank(raw_count, r)[rank * n + b];
-                if (need_mass) m += cluster.map_shared_rank(raw_mass, r)[rank * n + b];
-            }
-            merged_count[level * n + b] = c;
-            merged_mass[level * n + b] = m;
+            for (int r = 0; r < ranks; ++r) c += cluster.map_shared_rank(raw_count, r)[rank * n + b];
+            counts[b] = c;
             c_all += c;
+        }
+        for (int b = tid; b < heavy; b += kThreads) {
+            u64 m = 0;
+            for (int r = 0; r < ranks; ++r) m += cluster.map_shared_rank(raw_mass, r)[rank * heavy + b];
+            masses[b] = m;
             m_all += m;
         }
         c_all = __reduce_add_sync(0xffffffffu, c_all);
@@ -205,7 +298,7 @@ struct Row {
                 m += sh.warp_u64[w];
             }
             sh.chunk_count[level] = c;
-            sh.chunk_mass[level] = m;
+            sh.chunk_mass[level] = m;  // (of level 0 not used: its shares of counts and masses differ)
         }
         cluster.sync();
     }
@@ -215,14 +308,15 @@ struct Row {
         return by_mass ? !(static_cast<double>(mass) < target) : count >= k;
     }
 
-    // Finds the bin of `level` where the cut lies; false when no bin reaches it.
+    // Finds the bin of `level` where the cut lies, from exact sums (by weight: level 1 only); false
+    // when no bin reaches it.
     __device__ bool find_bin(int level, bool by_mass, unsigned k, double target, unsigned count, u64 mass) {
-        const int n = kBins / ranks;
+        const int n = bins_of(level) / ranks;
         int owner = -1;
         for (int r = 0; r < ranks; ++r) {
             const Shared* other = cluster.map_shared_rank(&sh, r);
             const unsigned c = other->chunk_count[level];
-            const u64 m = other->chunk_mass[level];
+            const u64 m = level == 1 ? other->chunk_mass[1] : 0ull;
             if (reached(by_mass, count + c, mass + m, k, target)) {
                 owner = r;
                 break;
@@ -231,8 +325,8 @@ struct Row {
             mass += m;
         }
         if (owner < 0) return false;
-        const unsigned* counts = cluster.map_shared_rank(merged_count, owner) + level * n;
-        const u64* masses = cluster.map_shared_rank(merged_mass, owner) + level * n;
+        const unsigned* counts = cluster.map_shared_rank(merged_count, owner) + (level == 0 ? 0 : kBins / ranks);
+        const u64* masses = cluster.map_shared_rank(merged_mass, owner) + kHeavyBins / ranks;
         // Each thread takes `per` consecutive bins.
         const int per = (n + kThreads - 1) / kThreads;
         unsigned c_mine = 0;
@@ -241,7 +335,7 @@ struct Row {
             const int b = tid * per + i;
             if (b < n) {
                 c_mine += counts[b];
-                m_mine += masses[b];
+                if (level == 1) m_mine += masses[b];
             }
         }
         unsigned c_in = c_mine;
@@ -266,14 +360,14 @@ struct Row {
         }
         unsigned c = count + c_in - c_mine;
         u64 m = mass + m_in - m_mine;
-        if (!reached(by_mass, c, m, k, target) || (c == 0 && m == 0)) {
+        if (!reached(by_mass, c, m, k, target)) {
             for (int i = 0; i < per; ++i) {
                 const int b = tid * per + i;
                 if (b >= n) break;
                 const unsigned tc = counts[b];
-                const u64 tm = masses[b];
+                const u64 tm = level == 1 ? masses[b] : 0ull;
                 if (tc != 0u && reached(by_mass, c + tc, m + tm, k, target)) {
-                    sh.bin = owner * n + b;
+                    sh.bin[0] = sh.bin[1] = owner * n + b;
                     sh.bin_count = tc;
                     sh.before_count = c;
                     sh.before_mass = m;
@@ -287,29 +381,124 @@ struct Row {
         return true;
     }
 
-    // The cut: the rank value of the last kept token (0 when all are kept), and in `kept` the
-    // weight up to it. Level 0 of the histogram has been merged.
-    __device__ u64 cut(bool by_mass, unsigned k, double target, u64& kept) {
-        if (!find_bin(0, by_mass, k, target, 0u, 0ull)) return 0ull;
+    // Finds the bins of level 0 where a cut by weight lies: an upper bound of the running weight has
+    // reached the target at the end of the first, and a lower bound at the end of the last. The first
+    // bins' weights are exact. Bounds of a later bin are its count times the weights of its edges
+    // where the window has to be `sure` to hold the cut (bins are 2^-7.2 wide; a margin of 2^-12 covers
+    // the bounds' own rounding), and its count times its middle weight, give or take 2^-11, where it
+    // will be checked.
+    __device__ void find_window(double target, bool sure) {
+        constexpr int kPer = kBins / kThreads;
+        const int n = kBins / ranks, heavy = kHeavyBins / ranks;
+        const float step = to_bin > 0.0f ? __fdividef(1.0f, to_bin * t) : 0.0f;
+        float near_[kPer], far_[kPer], near_sum = 0.0f, far_sum = 0.0f;
+        unsigned counts[kPer];
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const int b = tid * kPer + i;
+            counts[i] = cluster.map_shared_rank(merged_count, b / n)[b % n];
+            if (b < kHeavyBins) {
+                near_[i] = far_[i] = static_cast<float>(cluster.map_shared_rank(merged_mass, b / heavy)[b % heavy]) * (1.0f / kUnits);
+            } else {
+                const float c = static_cast<float>(counts[i]), at = static_cast<float>(b);
+                near_[i] = c * expf(-step * (sure ? at - 0.5f : at)) * (sure ? 1.0f : 1.0f + 0x1p-11f);
+                far_[i] = c * expf(-step * (sure ? at + 0.5f : at)) * (sure ? 1.0f : 1.0f - 0x1p-11f);
+            }
+            near_sum += near_[i];
+            far_sum += far_[i];
+        }
+        float near_in = near_sum, far_in = far_sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const float a = __shfl_up_sync(0xffffffffu, near_in, o), b = __shfl_up_sync(0xffffffffu, far_in, o);
+            if (lane >= o) {
+                near_in += a;
+                far_in += b;
+            }
+        }
+        if (lane == 31) {
+            sh.warp_f32[0][warp] = near_in;
+            sh.warp_f32[1][warp] = far_in;
+        }
+        if (tid == 0) {
+            sh.bin[0] = kBins - 1;
+            sh.bin[1] = kBins - 1;
+        }
+        __syncthreads();
+        for (int w = 0; w < warp; ++w) {
+            near_in += sh.warp_f32[0][w];
+            far_in += sh.warp_f32[1][w];
+        }
+        const float goal = static_cast<float>(target / static_cast<double>(kUnits));
+        const float above = sure ? 1.0f + 0x1p-12f : 1.0f + 0x1p-18f, below = sure ? 1.0f - 0x1p-12f : 1.0f - 0x1p-18f;
+        float a = near_in - near_sum, b = far_in - far_sum;
+        // Running sums only grow, so exactly one bin is the first to reach the goal. (Sums of other
+        // threads' bins may round differently here and there: the margin covers it, and the window
+        // is taken by minimum and maximum.)
+        int lo = kBins, hi = kBins;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            a += near_[i];
+            b += far_[i];
+            if (lo == kBins && a * above >= goal) lo = tid * kPer + i;
+            if (hi == kBins && b * below >= goal) hi = tid * kPer + i;
+        }
+        atomicMin(&sh.bin[0], lo);
+        atomicMin(&sh.bin[1], hi);
+        __syncthreads();
+        const int b0 = sh.bin[0], b1 = max(sh.bin[1], b0);
+        // Tokens before the window and in it.
+        unsigned before = 0u, in = 0u;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const int bin = tid * kPer + i;
+            if (bin < b0) before += counts[i];
+            if (bin >= b0 && bin <= b1) in += counts[i];
+        }
+        before = __reduce_add_sync(0xffffffffu, before);
+        in = __reduce_add_sync(0xffffffffu, in);
+        if (tid == 0) sh.before_count = sh.bin_count = 0u;
+        __syncthreads();
+        if (lane == 0) {
+            atomicAdd(&sh.before_count, before);
+            atomicAdd(&sh.bin_count, in);
+        }
+        if (tid == 0) sh.bin[1] = b1;
+        __syncthreads();
+    }
+
+    // The cut by count (top-k) or weight (top-p). Level 0 of the histogram has been merged.
+    __device__ Limit cut(bool by_mass, unsigned k, double target) {
+        if (by_mass) {
+            find_window(target, true);
+        } else if (!find_bin(0, false, k, target, 0u, 0ull)) {
+            return {-INFINITY, 0};
+        }
         int level = 0;
-        int bin = sh.bin;
+        int bin0 = sh.bin[0], bin1 = sh.bin[1];
         unsigned members = sh.bin_count, before_count = sh.before_count;
-        u64 before_mass = sh.before_mass;
-        u64 hi = 0ull, lo = 0ull;  // rank values of the bin's members, from level 1 on
-        while (members > static_cast<unsigned>(kList)) {
-            if (level == 0) {
-                u64 a = 0ull, b = ~0ull;
-                each([&](float x, int id) {
-                    const float d = distance(x);
-                    if (d <= spread && bin_of(d) == bin) {
-                        const u64 v = rank_value(x, id);
-                        a = v > a ? v : a;
-                        b = v < b ? v : b;
-                    }
-                });
+        u64 before_mass = 0ull;
+        u64 hi = 0ull, lo = 0ull;  // rank values of the listed bins' tokens, from level 1 on
+        const bool refine = members > static_cast<unsigned>(kOwnList);
+        if (refine || by_mass) {
+            // The weight before the window, and where its rank values lie.
+            u64 a = 0ull, b = ~0ull, mine = 0ull;
+            each([&](float x, int id) {
+                const float d = distance(x);
+                if (!(d <= spread)) return;
+                const int bin = bin_of(d);
+                if (bin > bin1) return;
+                if (bin < bin0) {
+                    if (by_mass) mine += weight(x);
+                } else if (refine) {
+                    const u64 v = rank_value(x, id);
+                    a = v > a ? v : a;
+                    b = v < b ? v : b;
+                }
+            });
+            if (refine) {
                 a = warp_max_u64(a);
                 b = ~warp_max_u64(~b);
-                __syncthreads();
                 if (tid == 0) {
                     sh.range_hi = 0ull;
                     sh.range_lo = ~0ull;
@@ -319,26 +508,31 @@ struct Row {
                     atomicMax(&sh.range_hi, a);
                     atomicMin(&sh.range_lo, b);
                 }
-                cluster.sync();
-                hi = 0ull;
-                lo = ~0ull;
+            }
+            before_mass = cluster_sum(mine, 1);
+            if (refine) {
                 for (int r = 0; r < ranks; ++r) {
                     const Shared* other = cluster.map_shared_rank(&sh, r);
-                    hi = max(hi, other->range_hi);
-                    lo = min(lo, other->range_lo);
+                    hi = r == 0 ? other->range_hi : max(hi, other->range_hi);
+                    lo = r == 0 ? other->range_lo : min(lo, other->range_lo);
                 }
             }
+        }
+        while (members > static_cast<unsigned>(kOwnList)) {
             const int bits = 64 - __clzll(static_cast<long long>(hi - lo) | 1ll);
-            const int shift = bits > 11 ? bits - 11 : 0;
-            clear_histogram();
+            const int shift = bits > 8 ? bits - 8 : 0;
+            clear_histogram(1);
             each([&](float x, int id) {
                 const u64 v = rank_value(x, id);
-                if (v <= hi && v >= lo) count(static_cast<int>((hi - v) >> shift), x);
+                if (v > hi || v < lo) return;
+                const int b = static_cast<int>((hi - v) >> shift);
+                atomicAdd(raw_count + b, 1u);
+                if (by_mass) atomicAdd(raw_mass + b, weight(x));
             });
             merge(1);
-            find_bin(1, by_mass, k, target, before_count, before_mass);
+            if (!find_bin(1, by_mass, k, target, before_count, before_mass)) return {-INFINITY, 0};
             level = 1;
-            bin = sh.bin;
+            const int bin = sh.bin[0];
             members = sh.bin_count;
             before_count = sh.before_count;
             before_mass = sh.before_mass;
@@ -347,56 +541,279 @@ struct Row {
             lo = hi - lo > width ? hi - width : lo;
             __syncthreads();
         }
-        // The bin's members, from all CTAs.
+        // The remaining tokens, from all CTAs. (At most kOwnList, so that a CTA's list holds them.)
         if (tid == 0) sh.listed = 0u;
         __syncthreads();
         each([&](float x, int id) {
             u64 v;
             if (level == 0) {
                 const float d = distance(x);
-                if (!(d <= spread) || bin_of(d) != bin) return;
+                if (!(d <= spread)) return;
+                const int bin = bin_of(d);
+                if (bin < bin0 || bin > bin1) return;
                 v = rank_value(x, id);
             } else {
                 v = rank_value(x, id);
                 if (v > hi || v < lo) return;
             }
-            const unsigned at = atomicAdd(&sh.listed, 1u);
-            own_list[at] = v;
-            own_list[kList + at] = need_mass ? weight(x) : 0ull;
+            append(v, by_mass ? weight(x) : 0ull);
         });
         cluster.sync();
+        const int n = copy_lists(true);
+        return ranked_cut(n, by_mass, k, target, before_count, before_mass);
+    }
+
+    // The cut among n listed tokens that follow before_count tokens of weight before_mass. The warps
+    // of the cluster share the tokens; the lanes of a warp share the others they are ranked against.
+    __device__ Limit ranked_cut(int n, bool by_mass, unsigned k, double target, unsigned before_count, u64 before_mass) {
+        if (tid == 0) sh.cut = 0ull;
+        cluster.sync();
+        for (int i = rank * kWarps + warp; i < n; i += ranks * kWarps) {
+            const u64 v = list[i];
+            unsigned c = 0u;
+            u64 m = 0ull;
+            for (int j = lane; j < n; j += 32) {
+                if (list[j] > v) {
+                    ++c;
+                    m += list[kList + j];
+                }
+            }
+            c = before_count + __reduce_add_sync(0xffffffffu, c);
+            m = before_mass + warp_sum_u64(m);
+            const u64 with = m + list[kList + i];
+            // Every token ranked at or before the one that reaches the cut is kept.
+            const bool open = by_mass ? (static_cast<double>(m) < target || c == 0) : c < k;
+            if (open && reached(by_mass, c + 1, with, k, target) && lane < ranks) *cluster.map_shared_rank(&sh.cut, lane) = v;
+        }
+        cluster.sync();  // the cut is known, and the lists are free again, in every CTA
+        const u64 last = sh.cut;
+        if (last == 0ull) return {-INFINITY, 0};
+        return {score_from_bits(static_cast<uint32_t>(last >> 32)), key_id(last)};
+    }
+
+    // A cut by weight in one pass over the slice, where the estimated window's tokens fit the lists
+    // and hold the cut: finds the limit and leaves every warp's kept weight (min-p applied) in
+    // sh.warp_u64.
+    __device__ bool cut_and_sum(double target, float min_p, Limit& limit) {
+        find_window(target, false);
+        if (sh.bin_count > static_cast<unsigned>(kList)) return false;
+        const int bin0 = sh.bin[0], bin1 = sh.bin[1];
+        const unsigned before_count = sh.before_count;
+        if (tid == 0) sh.listed = 0u;
+        __syncthreads();
+        // Logits above `surely` are in bins before the window, those below `least` behind it (a bin
+        // of margin and directed rounding for the edges); between them the bins decide.
+        const float least = to_bin > 0.0f ? __fsub_rd(top, (static_cast<float>(bin1) + 1.5f) / to_bin) : -FLT_MAX;
+        const float surely = to_bin > 0.0f ? __fsub_ru(top, (static_cast<float>(bin0) - 1.5f) / to_bin) : INFINITY;
+        const int share = p.slice / kWarps;
+        u64 all = 0ull, kept = 0ull;
+#pragma unroll 1
+        for (int base = warp * share; base < (warp + 1) * share; base += 32 * V::kN) {
+            const uint4 v = *reinterpret_cast<const uint4*>(data + base + lane * V::kN);
+            if (!(V::highest(v, -INFINITY) >= least)) continue;
+            float x[V::kN];
+            V::unpack(v, x);
+            int all_hi = 0, all_lo = 0, kept_hi = 0, kept_lo = 0;
+#pragma unroll
+            for (int i = 0; i < V::kN; ++i) {
+                if (!(x[i] >= least)) continue;
+                bool before = x[i] > surely;
+                if (!before) {
+                    const float d = distance(x[i]);
+                    const int bin = d <= spread ? bin_of(d) : kBins;
+                    before = bin < bin0;
+                    if (bin >= bin0 && bin <= bin1) append(rank_value(x[i], first + base + lane * V::kN + i), 0ull);
+                }
+                if (before) {
+                    const float e = share_of(x[i]);
+                    add_units(e, all_hi, all_lo);
+                    if (e >= min_p) add_units(e, kept_hi, kept_lo);
+                }
+            }
+            all += units(all_hi, all_lo);
+            kept += units(kept_hi, kept_lo);
+        }
+        const u64 before_mass = cluster_sum(all, 1);
+        unsigned most = 0u, n = 0u;
+        for (int r = 0; r < ranks; ++r) {
+            const unsigned c = cluster.map_shared_rank(&sh, r)->listed;
+            most = max(most, c);
+            n += c;
+        }
+        if (most > static_cast<unsigned>(kOwnList) || n > static_cast<unsigned>(kList)) {
+            cluster.sync();  // every CTA has read the counts
+            return false;
+        }
+        const int own = static_cast<int>(sh.listed);
+        for (int i = tid; i < own; i += kThreads) {
+            own_list[kOwnList + i] = weight(score_from_bits(static_cast<uint32_t>(own_list[i] >> 32)));
+        }
+        cluster.sync();
+        limit = ranked_cut(copy_lists(true), true, 0u, target, before_count, before_mass);
+        if (limit.x == -INFINITY) return false;  // the cut is not in the window
+        // The kept ones of the window, each to the warp that holds it.
+        kept = warp_sum_u64(kept);
+        __syncthreads();
+        if (lane == 0) sh.warp_u64[warp] = kept;
+        __syncthreads();
+        for (int i = tid; i < own; i += kThreads) {
+            const float x = score_from_bits(static_cast<uint32_t>(own_list[i] >> 32));
+            const int id = key_id(own_list[i]);
+            if (limit.keeps(x, id) && share_of(x) >= min_p) atomicAdd(&sh.warp_u64[(id - first) / share], own_list[kOwnList + i]);
+        }
+        __syncthreads();
+        return true;
+    }
+
+    // One more token for this CTA's list; entries past its capacity are only counted.
+    __device__ __forceinline__ void append(u64 v, u64 w) {
+        const unsigned at = atomicAdd(&sh.listed, 1u);
+        if (at < static_cast<unsigned>(kOwnList)) {
+            own_list[at] = v;
+            own_list[kOwnList + at] = w;
+        }
+    }
+
+    // Copies the lists of all CTAs, whose tokens together fit one, into this CTA's; their number.
+    __device__ int copy_lists(bool weights) {
         int n = 0;
         for (int r = 0; r < ranks; ++r) {
             const int m = static_cast<int>(cluster.map_shared_rank(&sh, r)->listed);
             const u64* theirs = cluster.map_shared_rank(own_list, r);
             for (int i = tid; i < m; i += kThreads) {
                 list[n + i] = theirs[i];
-                list[kList + n + i] = theirs[kList + i];
+                if (weights) list[kList + n + i] = theirs[kOwnList + i];
             }
             n += m;
         }
         __syncthreads();
-        for (int i = tid; i < n; i += kThreads) {
-            const u64 v = list[i];
-            unsigned c = before_count;
-            u64 m = before_mass;
-            for (int j = 0; j < n; ++j) {
-                if (list[j] > v) {
-                    ++c;
-                    m += list[kList + j];
-                }
+        return n;
+    }
+
+    // A lower bound of the k-th largest of the threads' values (1 <= k <= kThreads) that shares its
+    // upper 16 bits: two digits of 8 bits.
+    __device__ uint32_t kth_largest(uint32_t key, unsigned k) {
+        uint32_t found = 0u, mask = 0u;
+#pragma unroll
+        for (int shift = 24; shift >= 16; shift -= 8) {
+            if (tid < 256) sh.digit[tid] = 0u;
+            __syncthreads();
+            if ((key & mask) == found) atomicAdd(&sh.digit[(key >> shift) & 255u], 1u);
+            __syncthreads();
+            // Every warp does the same: lane l takes digits 255 - 8 l downwards.
+            unsigned c[8], sum = 0u;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                c[i] = sh.digit[255 - 8 * lane - i];
+                sum += c[i];
             }
-            const u64 with = m + list[kList + i];
-            // Every token of the bin ranked at or before the one that reaches the cut is kept.
-            const bool open = by_mass ? (static_cast<double>(m) < target || c == 0) : c < k;
-            if (open && reached(by_mass, c + 1, with, k, target)) {
-                sh.cut = v;
-                sh.cut_mass = with;
+            unsigned upto = sum;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const unsigned v = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += v;
+            }
+            unsigned before = upto - sum, pick = 0u, rest = 0u;
+            const bool mine = before < k && upto >= k;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (mine && before < k && before + c[i] >= k) {
+                    pick = 255 - 8 * lane - i;
+                    rest = k - before;
+                }
+                before += c[i];
+            }
+            const int owner = __ffs(__ballot_sync(0xffffffffu, mine)) - 1;
+            found |= __shfl_sync(0xffffffffu, pick, owner) << shift;
+            mask |= 255u << shift;
+            k = __shfl_sync(0xffffffffu, rest, owner);
+            __syncthreads();
+        }
+        return found;
+    }
+
+    // Top-k, top-p, min-p and the draw from n listed tokens that hold the top k. All CTAs rank, the
+    // first one draws.
+    __device__ void draw_from_list(int row, int n, unsigned k, float top_p, float min_p) {
+        // The k ranked first, in their order, in the first CTA: where its copy of the list's weights
+        // would be (none were listed).
+        u64* ranked = list + kList;  // [2][kDirect]
+        u64* there = cluster.map_shared_rank(ranked, 0);
+        for (int i = rank * kWarps + warp; i < n; i += ranks * kWarps) {
+            const u64 v = list[i];
+            unsigned c = 0u;
+            for (int j = lane; j < n; j += 32) c += list[j] > v ? 1u : 0u;
+            c = __reduce_add_sync(0xffffffffu, c);
+            if (c < k && lane == 0) {
+                there[c] = v;
+                there[kDirect + c] = weight(score_from_bits(static_cast<uint32_t>(v >> 32)));
             }
         }
-        cluster.sync();  // the lists are free again in every CTA
-        kept = sh.cut_mass;
-        return sh.cut;
+        cluster.sync();
+        if (rank != 0) return;
+        const int m = min(n, static_cast<int>(k));
+        // One warp: running weights in rank order (8 tokens a lane), then the filters.
+        if (warp == 0) {
+            constexpr int kPer = kDirect / 32;
+            u64 w[kPer], sum = 0ull;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                w[i] = lane * kPer + i < m ? ranked[kDirect + lane * kPer + i] : 0ull;
+                sum += w[i];
+            }
+            u64 upto = sum;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const u64 v = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += v;
+            }
+            const u64 all = __shfl_sync(0xffffffffu, upto, 31);
+            const double target = static_cast<double>(top_p) * static_cast<double>(all);
+            u64 before = upto - sum;
+            u64 kept_mass = 0ull;
+            unsigned kept = 0u;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                const int r = lane * kPer + i;
+                if (r < m) {
+                    const float x = score_from_bits(static_cast<uint32_t>(ranked[r] >> 32));
+                    const bool keep = r == 0 || ((!(top_p < 1.0f) || static_cast<double>(before) < target) && share_of(x) >= min_p);
+                    if (keep) {
+                        ++kept;
+                        kept_mass += w[i];
+                    }
+                }
+                before += w[i];
+            }
+            kept = __reduce_add_sync(0xffffffffu, kept);  // kept tokens are the first ones
+            kept_mass = warp_sum_u64(kept_mass);
+            if (lane == 0) {
+                sh.kept = static_cast<int>(kept);
+                sh.weight[0] = kept_mass;
+            }
+        }
+        __syncthreads();
+        const u64 total = sh.weight[0];
+        const u64 target = drawn(row, total);
+        if (tid < sh.kept) {
+            const int id = key_id(ranked[tid]);
+            u64 before = 0ull;
+            for (int j = 0; j < sh.kept; ++j) before += key_id(ranked[j]) < id ? ranked[kDirect + j] : 0ull;
+            const u64 w = ranked[kDirect + tid];
+            if (target >= before && target < before + w) write(row, id, w, total);
+        }
+    }
+
+    __device__ __forceinline__ u64 drawn(int row, u64 total) const {
+        float u = p.uniforms[row];
+        u = u >= 0.0f ? fminf(u, 0.99999994f) : 0.0f;
+        const u64 target = static_cast<u64>(floor(static_cast<double>(u) * static_cast<double>(total)));
+        return target >= total ? total - 1ull : target;
+    }
+
+    __device__ __forceinline__ void write(int row, int id, u64 w, u64 total) const {
+        p.tokens[row] = id;
+        if (p.logprobs != nullptr) p.logprobs[row] = static_cast<float>(log(static_cast<double>(w) / static_cast<double>(total)));
     }
 
     __device__ void run();
@@ -409,8 +826,16 @@ __device__ void Row<T>::run() {
     const int have = max(0, min(p.slice, p.vocab - first));
     const int share = p.slice / kWarps;
 
-    // ---- load, maximum and minimum ----
-    float hi = -INFINITY, lo = INFINITY;
+    t = p.temperature != nullptr ? p.temperature[row] : 1.0f;
+    const unsigned k = p.top_k != nullptr && p.top_k[row] > 0 ? static_cast<unsigned>(p.top_k[row]) : 0u;
+    const float top_p = p.top_p != nullptr ? p.top_p[row] : 1.0f;
+    float min_p = p.min_p != nullptr ? p.min_p[row] : 0.0f;
+    if (!(min_p > 0.0f)) min_p = 0.0f;
+    const bool only_first = !(t > 0.0f) || k == 1u || top_p <= 0.0f || min_p > 1.0f;
+    const bool direct = !only_first && k != 0u && k <= static_cast<unsigned>(kDirect);
+
+    // ---- load and maximum ----
+    float hi = -INFINITY;  // of this thread
     const bool wide = (reinterpret_cast<uintptr_t>(src) & 15u) == 0;
 #pragma unroll 4
     for (int at = warp * share + lane * V::kN; at < (warp + 1) * share; at += 32 * V::kN) {
@@ -422,42 +847,34 @@ __device__ void Row<T>::run() {
 #pragma unroll
             for (int i = 0; i < V::kN; ++i) e[i] = at + i < have ? src[at + i] : V::lowest();
         }
-        float x[V::kN];
-        V::unpack(v, x);
-#pragma unroll
-        for (int i = 0; i < V::kN; ++i) {
-            if (x[i] != x[i]) {  // NaN: never drawn
-                e[i] = V::lowest();
-                x[i] = -INFINITY;
-            }
-            hi = fmaxf(hi, x[i]);
-            if (x[i] != -INFINITY) lo = fminf(lo, x[i]);
-        }
+        hi = V::highest(v, hi);
         *reinterpret_cast<uint4*>(data + at) = v;
     }
-    hi = warp_max_f32(hi);
-    lo = -warp_max_f32(-lo);
-    if (lane == 0) {
-        sh.warp_f32[0][warp] = hi;
-        sh.warp_f32[1][warp] = lo;
-    }
-    __syncthreads();
-    if (tid == 0) {
-        for (int w = 0; w < kWarps; ++w) {
-            hi = fmaxf(hi, sh.warp_f32[0][w]);
-            lo = fminf(lo, sh.warp_f32[1][w]);
+    {
+        const float mine = hi;
+        hi = warp_max_f32(hi);
+        if (lane == 0) sh.warp_f32[0][warp] = hi;
+        __syncthreads();
+        float bound = -INFINITY;
+        if (direct) {
+            bound = score_from_bits(kth_largest(orderable_bits(mine), (k + ranks - 1) / ranks));
+            if (!(bound >= -FLT_MAX)) bound = -FLT_MAX;  // of -inf, or a NaN by the truncation: keeps all
         }
-        sh.top = hi;
-        sh.low = lo;
-        sh.best = 0ull;
+        if (tid == 0) {
+            for (int w = 0; w < kWarps; ++w) hi = fmaxf(hi, sh.warp_f32[0][w]);
+            sh.top = hi;
+            sh.bound = bound;
+            sh.best = 0ull;
+            sh.listed = 0u;
+        }
     }
     cluster.sync();
     top = -INFINITY;
-    lo = INFINITY;
+    float bound = INFINITY;
     for (int r = 0; r < ranks; ++r) {
         const Shared* other = cluster.map_shared_rank(&sh, r);
         top = fmaxf(top, other->top);
-        lo = fminf(lo, other->low);
+        bound = fminf(bound, other->bound);
     }
     if (top == -INFINITY) {
         if (rank == 0 && tid == 0) {
@@ -467,13 +884,7 @@ __device__ void Row<T>::run() {
         return;
     }
 
-    t = p.temperature != nullptr ? p.temperature[row] : 1.0f;
-    unsigned k = p.top_k != nullptr && p.top_k[row] > 0 ? static_cast<unsigned>(p.top_k[row]) : 0u;
-    float top_p = p.top_p != nullptr ? p.top_p[row] : 1.0f;
-    float min_p = p.min_p != nullptr ? p.min_p[row] : 0.0f;
-    if (!(min_p > 0.0f)) min_p = 0.0f;
-    if (!(t > 0.0f) || k == 1u || top_p <= 0.0f || min_p > 1.0f) {
-        // Only the first ranked token is kept.
+    if (only_first) {
         u64 best = 0ull;
         each([&](float x, int id) {
             if (x == top) best = max(best, rank_value(x, id));
@@ -489,54 +900,105 @@ __device__ void Row<T>::run() {
         return;
     }
 
-    u64 limit = 0ull;  // kept: rank value >= limit
-    need_mass = top_p < 1.0f;
-    if (need_mass || k != 0u) {
-        spread = fminf(top - lo, kWeightless * t);
-        if (!(spread > 0.0f)) spread = 0.0f;
-        to_bin = spread > 0.0f ? fminf((kBins - 0.01f) / spread, 1e30f) : 0.0f;
-        clear_histogram();
-        each([&](float x, int) {
-            const float d = distance(x);
-            if (d <= spread) count(bin_of(d), x);
-        });
+    // 0: t is out of the range where its reciprocal and the quotients' remainders are normal.
+    per_t = t > 0x1p-60f && t < 0x1p60f && top < INFINITY ? __frcp_rn(t) : 0.0f;
+
+    if (direct) {
+        each_from(bound, [&](float x, int id) { append(rank_value(x, id), 0ull); });
+        cluster.sync();
+        unsigned n = 0u, most = 0u;
+        for (int r = 0; r < ranks; ++r) {
+            const unsigned c = cluster.map_shared_rank(&sh, r)->listed;
+            most = max(most, c);
+            n += c;
+        }
+        if (most <= static_cast<unsigned>(kOwnList) && n <= static_cast<unsigned>(kList)) {
+            draw_from_list(row, copy_lists(false), k, top_p, min_p);
+            return;
+        }
+        cluster.sync();  // every CTA has read the counts
+    }
+
+    Limit limit{-INFINITY, 0};
+    const bool by_weight = top_p < 1.0f;
+    bool summed = false;  // the kept weights are in sh.warp_u64
+    if (by_weight || k != 0u) {
+        spread = kWeightless * t;
+        to_bin = fminf((kBins - 1) / spread, 1e30f);
+        clear_histogram(0);
+        u64 all = 0ull;
+        if (by_weight && k == 0u) {
+            // Counts and the total weight.
+#pragma unroll 1
+            for (int at = warp * share + lane * V::kN; at < (warp + 1) * share; at += 32 * V::kN) {
+                float x[V::kN];
+                V::unpack(*reinterpret_cast<const uint4*>(data + at), x);
+                int sum_hi = 0, sum_lo = 0;
+#pragma unroll
+                for (int i = 0; i < V::kN; ++i) {
+                    const float d = distance(x[i]);
+                    if (d <= spread && x[i] > -INFINITY) {
+                        const int bin = bin_of(d);
+                        const float e = share_of(x[i]);
+                        atomicAdd(raw_count + bin, 1u);
+                        if (bin < kHeavyBins) atomicAdd(raw_mass + bin, static_cast<u64>(__float2ll_rn(e * kUnits)));
+                        add_units(e, sum_hi, sum_lo);
+                    }
+                }
+                all += units(sum_hi, sum_lo);
+            }
+        } else {
+            each([&](float x, int) {
+                const float d = distance(x);
+                if (!(d <= spread)) return;
+                const int bin = bin_of(d);
+                atomicAdd(raw_count + bin, 1u);
+                if (by_weight && bin < kHeavyBins) atomicAdd(raw_mass + bin, weight(x));
+            });
+        }
         merge(0);
-        u64 total = 0ull;
-        for (int r = 0; r < ranks; ++r) total += cluster.map_shared_rank(&sh, r)->chunk_mass[0];
-        if (k != 0u) limit = cut(false, k, 0.0, total);
-        if (need_mass) {
-            const u64 l = cut(true, 0u, static_cast<double>(top_p) * static_cast<double>(total), total);
-            limit = max(limit, l);
+        if (k != 0u) limit = cut(false, k, 0.0);
+        if (by_weight) {
+            if (k != 0u) {
+                each_from(fmaxf(limit.x, -FLT_MAX), [&](float x, int id) {
+                    if (limit.keeps(x, id)) all += weight(x);
+                });
+            }
+            const u64 total = cluster_sum(all, 0);
+            const double target = static_cast<double>(top_p) * static_cast<double>(total);
+            // (Below the top-k's total weight, so the cut is not behind the top-k's.)
+            summed = cut_and_sum(target, min_p, limit);
+            if (!summed) limit = cut(true, 0u, target);
         }
     }
 
     // ---- the kept weight, in ascending id order ----
     u64 mine = 0ull;
-    each([&](float x, int id) {
-        if (rank_value(x, id) < limit) return;
-        const float e = share_of(x);
-        if (e >= min_p) mine += static_cast<u64>(__float2ll_rn(e * kUnits));
-    });
-    mine = warp_sum_u64(mine);
-    __syncthreads();
-    if (lane == 0) sh.warp_u64[warp] = mine;
-    __syncthreads();
+    if (!summed) {
+        each_from(fmaxf(limit.x, -FLT_MAX), [&](float x, int id) {
+            if (!limit.keeps(x, id)) return;
+            const float e = share_of(x);
+            if (e >= min_p) mine += static_cast<u64>(__float2ll_rn(e * kUnits));
+        });
+        mine = warp_sum_u64(mine);
+        __syncthreads();
+        if (lane == 0) sh.warp_u64[warp] = mine;
+        __syncthreads();
+    }
+    mine = sh.warp_u64[warp];
     if (tid == 0) {
         u64 all = 0ull;
         for (int w = 0; w < kWarps; ++w) all += sh.warp_u64[w];
-        sh.weight = all;
+        sh.weight[0] = all;
     }
     cluster.sync();
     u64 total = 0ull, before = 0ull;
     for (int r = 0; r < ranks; ++r) {
-        const u64 w = cluster.map_shared_rank(&sh, r)->weight;
+        const u64 w = cluster.map_shared_rank(&sh, r)->weight[0];
         if (r < rank) before += w;
         total += w;
     }
-    float u = p.uniforms[row];
-    u = u >= 0.0f ? fminf(u, 0.99999994f) : 0.0f;
-    u64 target = static_cast<u64>(floor(static_cast<double>(u) * static_cast<double>(total)));
-    if (target >= total) target = total - 1ull;
+    const u64 target = drawn(row, total);
     for (int w = 0; w < warp; ++w) before += sh.warp_u64[w];
     if (target < before || target >= before + mine) return;
     for (int base = warp * share; base < (warp + 1) * share; base += 32 * V::kN) {
@@ -547,7 +1009,7 @@ __device__ void Row<T>::run() {
 #pragma unroll
         for (int i = 0; i < V::kN; ++i) {
             w[i] = 0ull;
-            if (x[i] != -INFINITY && rank_value(x[i], first + at + i) >= limit) {
+            if (x[i] > -INFINITY && limit.keeps(x[i], first + at + i)) {
                 const float e = share_of(x[i]);
                 if (e >= min_p) w[i] = static_cast<u64>(__float2ll_rn(e * kUnits));
             }
@@ -565,12 +1027,7 @@ __device__ void Row<T>::run() {
             if (target >= at_mine && target < at_mine + sum) {
 #pragma unroll
                 for (int i = 0; i < V::kN; ++i) {
-                    if (target >= at_mine && target < at_mine + w[i]) {
-                        p.tokens[row] = first + at + i;
-                        if (p.logprobs != nullptr) {
-                            p.logprobs[row] = static_cast<float>(log(static_cast<double>(w[i]) / static_cast<double>(total)));
-                        }
-                    }
+                    if (target >= at_mine && target < at_mine + w[i]) write(row, first + at + i, w[i], total);
                     at_mine += w[i];
                 }
             }
@@ -580,13 +1037,17 @@ __device__ void Row<T>::run() {
     }
 }
 
-// Shared memory after the slice: [histogram | own list and list share it] [merged, two levels].
-constexpr size_t kWorkBytes = 4ull * kList * 8 > 12ull * kBins ? 4ull * kList * 8 : 12ull * kBins;
+// Shared memory after the slice: [own list and list | the histogram shares it] [merged bins].
+constexpr size_t kListBytes = 16ull * kOwnList + 16ull * kList;
+constexpr size_t kWorkBytes = kListBytes;
+static_assert(kListBytes >= 4ull * kBins + 8ull * kHeavyBins, "the histogram shares the lists' memory");
 
-size_t smem_bytes(int slice, int cluster, size_t element) { return slice * element + kWorkBytes + 2ull * (kBins / cluster) * 12; }
+size_t smem_bytes(int slice, int cluster, size_t element) {
+    return slice * element + kWorkBytes + 8ull * ((kHeavyBins + kSubBins) / cluster) + 4ull * ((kBins + kSubBins) / cluster);
+}
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) {
+__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleParams p) {
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ Shared sh;
     Row<T> row(p, sh);
@@ -599,11 +1060,11 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleParams p) 
     row.data = reinterpret_cast<T*>(smem);
     uint8_t* work = smem + static_cast<size_t>(p.slice) * sizeof(T);
     row.raw_mass = reinterpret_cast<u64*>(work);
-    row.raw_count = reinterpret_cast<unsigned*>(work + 8 * kBins);
+    row.raw_count = reinterpret_cast<unsigned*>(work + 8 * kHeavyBins);
     row.own_list = reinterpret_cast<u64*>(work);
-    row.list = row.own_list + 2 * kList;
+    row.list = row.own_list + 2 * kOwnList;
     row.merged_mass = reinterpret_cast<u64*>(work + kWorkBytes);
-    row.merged_count = reinterpret_cast<unsigned*>(row.merged_mass + 2 * (kBins / row.ranks));
+    row.merged_count = reinterpret_cast<unsigned*>(row.merged_mass + (kHeavyBins + kSubBins) / row.ranks);
     row.run();
     row.cluster.sync();  // no CTA leaves while another may still read its shared memory
 }
@@ -619,11 +1080,12 @@ int launch(const SampleParams& base, int rows, cudaStream_t stream) {
     const auto kernel = sample_kernel<T>;
     cudaError_t e = ensure_smem_optin(reinterpret_cast<const void*>(kernel));
     if (e != cudaSuccess) return fail_cuda(e, "zcgvs_sample");
-    const size_t limit = static_cast<size_t>(device_max_smem()) - sizeof(Shared) - 1024;
-    // CTAs per row: enough to hold the row, then more while the rows leave SMs idle and a CTA
-    // still has 4096 tokens.
+    // An SM has 1024 bytes more than one CTA may take, and every CTA costs 1024 on top.
+    const size_t half = (static_cast<size_t>(device_max_smem()) + 1024) / 2 - sizeof(Shared) - 1024;
+    // CTAs per row: enough that two of them fit an SM where that is possible (one always fits),
+    // then more while the rows leave SMs idle and a CTA still has 4096 tokens.
     int cluster = 1;
-    while (cluster < kMaxCluster && smem_bytes(slice_of(base.vocab, cluster), cluster, sizeof(T)) > limit) cluster *= 2;
+    while (cluster < kMaxCluster && smem_bytes(slice_of(base.vocab, cluster), cluster, sizeof(T)) > half) cluster *= 2;
     while (cluster < kMaxCluster && static_cast<long long>(rows) * cluster * 2 <= device_sm_count() && base.vocab / (cluster * 2) >= 4096) {
         cluster *= 2;
     }
