@@ -231,6 +231,23 @@ struct Row {
     __device__ __forceinline__ static u64 units(int hi, int lo) {
         return static_cast<u64>((static_cast<long long>(hi) << 20) + lo);
     }
+    // share_of and add_units of two tokens by their a = x - m >= floor_ (two operations an
+    // instruction), where per_t is set; weights at floor_ are 0.
+    __device__ __forceinline__ float2 shares2(float2 a) const {
+        const float2 y = both(per_t), minus_t = both(-t);
+        float2 q = fma2(a, y, both(0.0f));
+        q = fma2(fma2(q, minus_t, a), y, q);
+        q = fma2(fma2(q, minus_t, a), y, q);
+        return make_float2(expf(q.x), expf(q.y));
+    }
+    __device__ __forceinline__ static void add_units2(float2 e, int& hi, int& lo) {
+        const float2 big = both(12582912.0f), unit = both(1048576.0f);
+        const float2 h = fma2(e, unit, big);
+        const float2 l = fma2(fma2(e, unit, fma2(h, both(-1.0f), big)), unit, big);
+        hi += (__float_as_int(h.x) - 0x4B400000) + (__float_as_int(h.y) - 0x4B400000);
+        lo += (__float_as_int(l.x) - 0x4B400000) + (__float_as_int(l.y) - 0x4B400000);
+    }
+
     // The bin of a distance at most `spread`: the nearest integer of d * to_bin.
     __device__ __forceinline__ int bin_of(float d) const {
         return min(kBins - 1, __float_as_int(fmaf(d, to_bin, 8388608.0f)) & 0x7FFFFF);
@@ -606,6 +623,7 @@ struct Row {
         const float least = to_bin > 0.0f ? __fsub_rd(top, (static_cast<float>(bin1) + 1.5f) / to_bin) : -FLT_MAX;
         const float surely = to_bin > 0.0f ? __fsub_ru(top, (static_cast<float>(bin0) - 1.5f) / to_bin) : INFINITY;
         const int share = p.slice / kWarps;
+        const float floor_ = -1.5f * spread;
         u64 all = 0ull, kept = 0ull;
 #pragma unroll 1
         for (int base = warp * share; base < (warp + 1) * share; base += 32 * V::kN) {
@@ -614,17 +632,38 @@ struct Row {
             float x[V::kN];
             V::unpack(v, x);
             int all_hi = 0, all_lo = 0, kept_hi = 0, kept_lo = 0;
+            // Where the bins decide: x becomes +inf before the window and -inf in it, listed, or behind.
+            bool near = false;
 #pragma unroll
-            for (int i = 0; i < V::kN; ++i) {
-                if (!(x[i] >= least)) continue;
-                bool before = x[i] > surely;
-                if (!before) {
-                    const float d = distance(x[i]);
-                    const int bin = d <= spread ? bin_of(d) : kBins;
-                    before = bin < bin0;
-                    if (bin >= bin0 && bin <= bin1) append(rank_value(x[i], first + base + lane * V::kN + i), 0ull);
+            for (int i = 0; i < V::kN; ++i) near |= x[i] >= least && !(x[i] > surely);
+            float raised[V::kN];
+#pragma unroll
+            for (int i = 0; i < V::kN; ++i) raised[i] = x[i];
+            if (near) {
+#pragma unroll
+                for (int i = 0; i < V::kN; ++i) {
+                    if (x[i] >= least && !(x[i] > surely)) {
+                        const float d = distance(x[i]);
+                        const int bin = d <= spread ? bin_of(d) : kBins;
+                        if (bin >= bin0 && bin <= bin1) append(rank_value(x[i], first + base + lane * V::kN + i), 0ull);
+                        raised[i] = bin < bin0 ? INFINITY : -INFINITY;
+                    }
                 }
-                if (before) {
+            }
+            auto before = [&](int i) { return raised[i] > surely; };
+            if (per_t != 0.0f) {
+#pragma unroll
+                for (int i = 0; i < V::kN; i += 2) {
+                    const bool b0 = before(i), b1 = before(i + 1);
+                    float2 e = add2(make_float2(x[i], x[i + 1]), both(-top));
+                    e = shares2(make_float2(b0 ? e.x : floor_, b1 ? e.y : floor_));
+                    add_units2(e, all_hi, all_lo);
+                    if (min_p > 0.0f) add_units2(make_float2(e.x >= min_p ? e.x : 0.0f, e.y >= min_p ? e.y : 0.0f), kept_hi, kept_lo);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < V::kN; ++i) {
+                    if (!before(i)) continue;
                     const float e = share_of(x[i]);
                     add_units(e, all_hi, all_lo);
                     if (e >= min_p) add_units(e, kept_hi, kept_lo);
@@ -633,6 +672,7 @@ struct Row {
             all += units(all_hi, all_lo);
             kept += units(kept_hi, kept_lo);
         }
+        if (per_t != 0.0f && !(min_p > 0.0f)) kept = all;
         const u64 before_mass = cluster_sum(all, 1);
         unsigned most = 0u, n = 0u;
         for (int r = 0; r < ranks; ++r) {
@@ -929,20 +969,37 @@ __device__ void Row<T>::run() {
         u64 all = 0ull;
         if (by_weight && k == 0u) {
             // Counts and the total weight.
+            const float floor_ = -1.5f * spread;
 #pragma unroll 1
             for (int at = warp * share + lane * V::kN; at < (warp + 1) * share; at += 32 * V::kN) {
                 float x[V::kN];
                 V::unpack(*reinterpret_cast<const uint4*>(data + at), x);
                 int sum_hi = 0, sum_lo = 0;
+                auto count = [&](float a, float e) {
+                    if (!(a >= -spread)) return;
+                    const int bin = bin_of(-a);
+                    atomicAdd(raw_count + bin, 1u);
+                    if (bin < kHeavyBins) atomicAdd(raw_mass + bin, static_cast<u64>(__float2ll_rn(e * kUnits)));
+                };
+                if (per_t != 0.0f) {
 #pragma unroll
-                for (int i = 0; i < V::kN; ++i) {
-                    const float d = distance(x[i]);
-                    if (d <= spread && x[i] > -INFINITY) {
-                        const int bin = bin_of(d);
+                    for (int i = 0; i < V::kN; i += 2) {
+                        // (fmaxf: -inf and NaN weigh nothing.)
+                        const float2 a = add2(make_float2(x[i], x[i + 1]), both(-top));
+                        const float2 b = make_float2(fmaxf(a.x, floor_), fmaxf(a.y, floor_));
+                        const float2 e = shares2(b);
+                        add_units2(e, sum_hi, sum_lo);
+                        count(b.x, e.x);
+                        count(b.y, e.y);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < V::kN; ++i) {
+                        const float d = distance(x[i]);
+                        if (!(d <= spread && x[i] > -INFINITY)) continue;
                         const float e = share_of(x[i]);
-                        atomicAdd(raw_count + bin, 1u);
-                        if (bin < kHeavyBins) atomicAdd(raw_mass + bin, static_cast<u64>(__float2ll_rn(e * kUnits)));
                         add_units(e, sum_hi, sum_lo);
+                        count(-d, e);
                     }
                 }
                 all += units(sum_hi, sum_lo);
