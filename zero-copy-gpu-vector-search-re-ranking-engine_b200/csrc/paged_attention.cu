@@ -10,9 +10,9 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
+#include <cstring>
 
 #include "paged_chunk.cuh"
-#include "paged_stream.cuh"
 
 namespace zc {
 namespace paged {
@@ -45,7 +45,10 @@ int padded(int head_dim) { return head_dim <= 64 ? 64 : 128; }
 
 constexpr int kStreamRows = 64;  // largest row tile of the streaming kernel
 
-int stream_ctas(int padded_dim, int sms) { return std::min(kMaxCtas, sms * (padded_dim == 64 ? stream_ctas_per_sm<64>() : stream_ctas_per_sm<128>())); }
+// The largest grid of the streaming kernel.
+int stream_ctas(int padded_dim, int sms) {
+    return std::min(kMaxCtas, sms * (padded_dim == 64 ? stream_ctas_per_sm<64, true>() : stream_ctas_per_sm<128, true>()));
+}
 
 int chunk_ctas(int sms) { return std::min(kMaxCtas, sms); }
 
@@ -61,31 +64,6 @@ uint32_t next_epoch() {
     uint32_t e = ++g_epoch;
     while (e == 0) e = ++g_epoch;  // 0 marks a ticket that was left at zero
     return e;
-}
-
-template <typename T, int DP, int WM>
-cudaError_t launch_stream(const AttnParams& p, int ctas, cudaStream_t stream) {
-    auto kernel = stream_kernel<T, DP, WM>;
-    const cudaError_t e = ensure_smem_optin(reinterpret_cast<const void*>(kernel));
-    if (e != cudaSuccess) return e;
-    KernelTimer timer("paged_stream", stream);
-    kernel<<<ctas, kStreamThreads, stream_stages<DP>() * stream_stage_bytes<DP>(), stream>>>(p);
-    return cudaGetLastError();
-}
-
-template <typename T, int DP>
-cudaError_t launch_stream_rows(const AttnParams& p, long long rows, int ctas, cudaStream_t stream) {
-    // The smallest row tile that holds a sequence's rows: fewer rows per warp leave warps to split
-    // the keys.
-    if (rows <= 16) return launch_stream<T, DP, 1>(p, ctas, stream);
-    if (rows <= 32) return launch_stream<T, DP, 2>(p, ctas, stream);
-    return launch_stream<T, DP, 4>(p, ctas, stream);
-}
-
-template <typename T>
-cudaError_t launch_stream_any(const AttnParams& p, long long rows, int ctas, cudaStream_t stream) {
-    return padded(p.view.head_dim) == 64 ? launch_stream_rows<T, 64>(p, rows, ctas, stream)
-                                         : launch_stream_rows<T, 128>(p, rows, ctas, stream);
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
@@ -132,21 +110,66 @@ bool make_query_map(CUtensorMap* map, const AttnParams& p, int dtype) {
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-struct ChunkMaps {
-    CUtensorMap keys, values, queries;
-    int box_log2 = 0;
-    int q_by_tma = 0;
+struct CacheMaps {
+    CUtensorMap keys, values;
+    int box_log2;
 };
 
-// Whether the chunk kernel can take this cache: pages made of whole groups of 8 slots (the
-// swizzle's), and strides a tensor map accepts.
-bool make_chunk_maps(const zcgvs_paged_cache& c, const AttnParams& p, ChunkMaps& maps) {
-    maps.q_by_tma = (p.group & (p.group - 1)) == 0 && p.group <= 128 && make_query_map(&maps.queries, p, c.dtype) ? 1 : 0;
+struct ChunkMaps {
+    CacheMaps cache;
+    CUtensorMap queries;
+    int q_by_tma;
+};
+
+// Maps with boxes of at most `keys` slots. False where a cache does not fit them: pages are made
+// of whole groups of 8 slots (the swizzle's), and strides are such as a tensor map accepts.
+bool make_cache_maps(const zcgvs_paged_cache& c, int keys, CacheMaps& maps) {
+    std::memset(&maps, 0, sizeof(maps));
     if (c.page_size % 8 != 0 || c.pages <= 0) return false;
     int log2 = 3;
-    while (log2 < 7 && c.page_size % (2 << log2) == 0) ++log2;
+    while ((2 << log2) <= keys && c.page_size % (2 << log2) == 0) ++log2;
     maps.box_log2 = log2;
     return make_cache_map(&maps.keys, c.keys, c, 1 << log2) && make_cache_map(&maps.values, c.values, c, 1 << log2);
+}
+
+// The same for the chunk kernel, with the queries' map where boxes fit the head groups.
+bool make_chunk_maps(const zcgvs_paged_cache& c, const AttnParams& p, ChunkMaps& maps) {
+    if (!make_cache_maps(c, kChunkKeys, maps.cache)) return false;
+    maps.q_by_tma = (p.group & (p.group - 1)) == 0 && p.group <= 128 && make_query_map(&maps.queries, p, c.dtype) ? 1 : 0;
+    if (!maps.q_by_tma) maps.queries = maps.cache.keys;  // not used
+    return true;
+}
+
+template <typename T, int DP, int WM, bool TMA>
+cudaError_t launch_stream(const AttnParams& p, const CacheMaps& maps, int sms, cudaStream_t stream) {
+    auto kernel = stream_kernel<T, DP, WM, TMA>;
+    const cudaError_t e = ensure_smem_optin(reinterpret_cast<const void*>(kernel));
+    if (e != cudaSuccess) return e;
+    KernelTimer timer("paged_stream", stream);
+    kernel<<<std::min(kMaxCtas, sms * stream_ctas_per_sm<DP, TMA>()), stream_threads<TMA>(), stream_smem_bytes<DP>(), stream>>>(
+        maps.keys, maps.values, p, maps.box_log2);
+    return cudaGetLastError();
+}
+
+template <typename T, int DP, bool TMA>
+cudaError_t launch_stream_rows(const AttnParams& p, const CacheMaps& maps, long long rows, int sms, cudaStream_t stream) {
+    // The smallest row tile that holds a sequence's rows: fewer rows per warp leave warps to split
+    // the keys.
+    if (rows <= 16) return launch_stream<T, DP, 1, TMA>(p, maps, sms, stream);
+    if (rows <= 32) return launch_stream<T, DP, 2, TMA>(p, maps, sms, stream);
+    return launch_stream<T, DP, 4, TMA>(p, maps, sms, stream);
+}
+
+template <typename T, int DP>
+cudaError_t launch_stream_dim(const AttnParams& p, const zcgvs_paged_cache& c, long long rows, int sms, cudaStream_t stream) {
+    CacheMaps maps;
+    return make_cache_maps(c, kStreamKeys, maps) ? launch_stream_rows<T, DP, true>(p, maps, rows, sms, stream)
+                                                 : launch_stream_rows<T, DP, false>(p, maps, rows, sms, stream);
+}
+
+template <typename T>
+cudaError_t launch_stream_any(const AttnParams& p, const zcgvs_paged_cache& c, long long rows, int sms, cudaStream_t stream) {
+    return padded(p.view.head_dim) == 64 ? launch_stream_dim<T, 64>(p, c, rows, sms, stream) : launch_stream_dim<T, 128>(p, c, rows, sms, stream);
 }
 
 template <typename T, int DP>
@@ -161,8 +184,8 @@ cudaError_t launch_chunk(const AttnParams& base, const ChunkMaps& maps, int ctas
     Join* joins = reinterpret_cast<Join*>(reinterpret_cast<uint8_t*>(p.status) + kJoinsAt);
     {
         KernelTimer timer("paged_chunk", stream);
-        kernel<<<ctas, kChunkThreads, chunk_smem_bytes<DP>(), stream>>>(maps.keys, maps.values, maps.q_by_tma ? maps.queries : maps.keys, p, joins,
-                                                                       maps.box_log2, maps.q_by_tma);
+        kernel<<<ctas, kChunkThreads, chunk_smem_bytes<DP>(), stream>>>(maps.cache.keys, maps.cache.values, maps.queries, p, joins,
+                                                                       maps.cache.box_log2, maps.q_by_tma);
     }
     cudaError_t launched = cudaGetLastError();
     if (launched != cudaSuccess) return launched;
@@ -269,8 +292,7 @@ int zcgvs_paged_attention(const zcgvs_paged_cache* cache, const zcgvs_step_batch
         p.epoch = next_epoch();
     }
     const long long stream_rows = std::min(rows, static_cast<long long>(p.rows_to));
-    const int ctas = stream_ctas(dim, sms);
-    const cudaError_t e = f16 ? launch_stream_any<__half>(p, stream_rows, ctas, s) : launch_stream_any<__nv_bfloat16>(p, stream_rows, ctas, s);
+    const cudaError_t e = f16 ? launch_stream_any<__half>(p, *cache, stream_rows, sms, s) : launch_stream_any<__nv_bfloat16>(p, *cache, stream_rows, sms, s);
     if (e != cudaSuccess) return fail_cuda(e, what);
     return ok();
 }

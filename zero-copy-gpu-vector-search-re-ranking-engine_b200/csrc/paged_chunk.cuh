@@ -33,7 +33,7 @@
 
 #include <type_traits>
 
-#include "paged_plan.cuh"
+#include "paged_stream.cuh"
 
 namespace zc {
 namespace paged {
@@ -145,24 +145,12 @@ __device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t* v) {
 }
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// One box of a cache map: 64 elements from x, box slots from `slot`, one head, one page.
+// 128 rows of queries: 64 elements from x, a head group, whole tokens.
 __device__ __forceinline__ void load_queries_box(uint32_t dst, const CUtensorMap* map, int x, int head, int token, u64* bar) {
     asm volatile(
         "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
         "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(head), "r"(token), "r"(smem_u32(bar))
         : "memory");
-}
-__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int x, int slot, int head, int page, u64* bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(slot), "r"(head), "r"(page), "r"(smem_u32(bar))
-        : "memory");
-}
-
-__device__ __forceinline__ float exp2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
 }
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -666,7 +654,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                         // Nothing seen yet: sum and this row of O are zero.
                         top = best;
                     } else if ((best - top) * scale > kRescaleAbove) {
-                        shrink = exp2_fast((top - best) * scale);
+                        shrink = exp2_approx((top - best) * scale);
                         top = best;
                     }
                     if (__any_sync(0xffffffffu, shrink != 1.0f)) {
@@ -695,7 +683,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
 #pragma unroll
                         for (int c = 0; c < 64; c += 2) {
                             const float2 x = fma2(make_float2(s[from + c], s[from + c + 1]), scale2, base2);
-                            const float2 w = make_float2(exp2_fast(x.x), exp2_fast(x.y));
+                            const float2 w = make_float2(exp2_approx(x.x), exp2_approx(x.y));
                             part[(c >> 1) & 1] = add2(part[(c >> 1) & 1], w);
                             packed[c >> 1] = pack2<T>(w.x, w.y);
                         }

@@ -4,49 +4,65 @@
 // used for few rows, and the time is that of reading them once: 2 * 2 * head_dim bytes per key
 // and head. The arithmetic (4 * head_dim operations per row and key) stays far below what the
 // warp-level tensor instructions (m16n8k16) deliver, so the kernel is built for a steady stream:
-// 4 warps take 64-key tiles from a ring of shared-memory stages that 16-byte asynchronous copies
-// fill ahead; each thread finds its rows' pages one tile ahead. Copies of keys outside the unit's
-// range are zero-filled, so nothing that lies in unused slots reaches the products. A row of 128
-// (or 64) elements is stored with its 16-byte pieces permuted by the row's low three bits, which
-// keeps the matrix loads free of bank conflicts.
-//
-// The 4 warps split a tile by rows (16 per warp) and, where the rows are fewer, by keys: with at
-// most 16 rows each warp takes 16 keys of the tile and keeps running maxima, sums and outputs of
-// its own, joined in shared memory at the end of the unit. No warp waits for another inside a
-// tile. Scores, maxima, sums and outputs are fp32; the weights are rounded to the cache's type
-// for the second product, as the instruction takes both operands in one type.
+//   * A producer warp keeps a ring of shared-memory slots filled with 64-key tiles of keys and
+//     values, by TMA loads from the pages (64 elements x the largest power of two of slots that a page
+//     holds whole, at most 64; 128-byte swizzle). It runs ahead over the ends of units. Pages that are
+//     not made of groups of 8 slots do not fit the swizzle: then four warps fill the ring with
+//     16-byte asynchronous copies.
+//   * 4 warps take the tiles. They split a tile by rows (16 per warp) and, where the rows are fewer,
+//     by keys: with at most 16 rows each warp takes 16 keys of the tile and keeps running maxima,
+//     sums and outputs of its own. No warp waits for another inside a unit; at its end the warps
+//     are joined through one more slot of the ring.
+// Value rows outside the unit's keys are cleared before they are used, so nothing that lies in
+// unused slots reaches the products. Scores, maxima, sums and outputs are fp32; the weights are
+// rounded to the cache's type for the second product, as the instruction takes both operands in
+// one type.
 #pragma once
+
+#include <cuda.h>
 
 #include "paged_plan.cuh"
 
 namespace zc {
 namespace paged {
 
-constexpr int kStreamThreads = 128;
+constexpr int kStreamWarps = 4;  // that compute
 constexpr int kStreamKeys = 64;  // keys per tile
-constexpr int kStreamExtra = 1;  // a unit's fill and end, in tiles
+constexpr int kStreamExtra = 1;  // a unit's end, in tiles
+constexpr int kStreamBarrier = 1;
+constexpr uint32_t kStatusStreamTile = kStatusTileWaitTimeout;
 
-template <int DP>
-constexpr int stream_stage_bytes() {
-    return 2 * kStreamKeys * DP * 2;
+template <bool TMA>
+constexpr int stream_producers() {
+    return TMA ? 1 : 4;
+}
+template <bool TMA>
+constexpr int stream_threads() {
+    return 32 * (kStreamWarps + stream_producers<TMA>());
 }
 template <int DP>
-constexpr int stream_stages() {
+constexpr int stream_slot_bytes() {
+    return 2 * kStreamKeys * DP * 2;  // the keys, then the values, each in columns of 64 elements
+}
+template <int DP>
+constexpr int stream_slots() {
     return DP == 128 ? 3 : 4;
 }
-
-template <int DP>
+template <int DP, bool TMA>
 constexpr int stream_ctas_per_sm() {
-    return DP == 128 ? 2 : 3;
+    return !TMA ? 1 : DP == 128 ? 2 : 3;
+}
+template <int DP>
+constexpr int stream_smem_bytes() {
+    return stream_slots<DP>() * stream_slot_bytes<DP>() + 1024;
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// One arrival on `bar` when the thread's copies so far have landed.
+__device__ __forceinline__ void cp_async_arrive(u64* bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
@@ -77,6 +93,26 @@ __device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&d)[4], const uin
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// One box of a cache map: 64 elements from x, its slots from `slot`, one head, one page.
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int x, int slot, int head, int page, u64* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(slot), "r"(head), "r"(page), "r"(smem_u32(bar))
+        : "memory");
+}
+
+// Named barrier over the computing warps that also ANDs a predicate across them.
+__device__ __forceinline__ bool stream_barrier(bool pred) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\t"
+        "bar.red.and.pred q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(r)
+        : "r"(pred ? 1 : 0), "n"(kStreamBarrier), "n"(32 * kStreamWarps)
+        : "memory");
+    return r != 0u;
+}
+
 __device__ __forceinline__ float exp2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -84,72 +120,151 @@ __device__ __forceinline__ float exp2_approx(float x) {
 }
 
 // WM warps over the rows (R = 16 WM), 4 / WM over the keys of a tile.
-template <typename T, int DP, int WM>
-__global__ void __launch_bounds__(kStreamThreads, stream_ctas_per_sm<DP>()) stream_kernel(const AttnParams p) {
+template <typename T, int DP, int WM, bool TMA>
+__global__ void __launch_bounds__(stream_threads<TMA>(), stream_ctas_per_sm<DP, TMA>())
+    stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const AttnParams p, int box_log2) {
     constexpr int R = 16 * WM;
-    constexpr int WK = 4 / WM;
+    constexpr int WK = kStreamWarps / WM;
     constexpr int KW = kStreamKeys / WK;  // keys of a tile per warp
-    constexpr int kStages = stream_stages<DP>();
-    constexpr int kPieces = DP / 8;              // 16-byte pieces of a row
-    constexpr int kRowsPerStep = kStreamThreads / kPieces;
-    constexpr int kSteps = kStreamKeys / kRowsPerStep;
-    constexpr int kLine = DP + 8;  // floats per row of the joining buffer
-    extern __shared__ __align__(1024) uint8_t smem[];
-    __shared__ PlanShared<kStreamThreads> plan_shared;
-    __shared__ int s_last;
+    constexpr int kSlots = stream_slots<DP>();
+    constexpr int kSlotBytes = stream_slot_bytes<DP>();
+    constexpr int kColumns = DP / 64;
+    constexpr int kColumnBytes = kStreamKeys * 128;
+    constexpr int kThreads = stream_threads<TMA>();
+    static_assert(WK * R * DP * 4 <= kSlotBytes, "a slot of the ring joins the warps");
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ PlanShared<kThreads> plan_shared;
+    __shared__ u64 s_full[kSlots], s_empty[kSlots];
+    __shared__ int s_last, s_abort;
     __shared__ float s_ml[WK][R][2];
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int wr = warp % WM, wk = warp / WM;
     const View& view = p.view;
-    const int d_pieces = view.head_dim / 8;
+    const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
 
-    Planner<R, kStreamKeys, kStreamThreads, 1, kStreamExtra> plan(p, plan_shared);
+    Planner<R, kStreamKeys, kThreads, 1, kStreamExtra> plan(p, plan_shared);
     if (!plan.start(1)) return;
+    if (tid == 0) {
+        for (int s = 0; s < kSlots; ++s) {
+            mbar_init(&s_full[s], TMA ? 1 : 32 * stream_producers<TMA>());
+            mbar_init(&s_empty[s], kStreamWarps);
+        }
+        fence_mbarrier_init();
+        s_abort = 0;
+    }
+    __syncthreads();
     Segment g = plan_shared.segment;
+    volatile int* abort_flag = &s_abort;
+    auto wait = [&](u64* bar, uint32_t parity) {
+        if (mbar_try_wait(smem_u32(bar), parity)) return true;
+        if (*abort_flag || !mbar_wait_bounded(bar, parity, p.status, kStatusStreamTile)) {
+            *abort_flag = 1;
+            return false;
+        }
+        return true;
+    };
 
-    const int my_piece = tid % kPieces, my_row = tid / kPieces;
-    const bool my_piece_valid = my_piece < d_pieces;
-    const uint32_t smem_base = smem_u32(smem);
+    if (warp >= kStreamWarps) {
+        // ---------------- producer ----------------
+        uint32_t used = 0;  // slots handed out
+        bool ok = true;
+        auto slot_empty = [&]() {
+            const uint32_t s = used % kSlots;
+            if (used >= kSlots) ok = __all_sync(0xffffffffu, wait(&s_empty[s], ((used / kSlots) - 1u) & 1u));
+            return ok;
+        };
+        if constexpr (TMA) {
+            // Lane: box of the tile (lane / (2 kColumns)), keys or values, 64-element column.
+            const int box = 1 << box_log2;
+            const int of_box = lane / (2 * kColumns), which = (lane / kColumns) & 1, column = lane % kColumns;
+            const uint32_t box_bytes = static_cast<uint32_t>(box) * 128u;
+            const uint32_t at = which * (kColumns * kColumnBytes) + column * kColumnBytes + of_box * box_bytes;
+            int page = -1, slot = 0;
+            bool mine = false;
+            auto find = [&](const Segment& of, int t) {
+                const int pos = (of.range.first + t) * kStreamKeys + of_box * box;
+                mine = of_box * box < kStreamKeys && pos < of.range.hi && pos + box > of.range.lo;
+                if (mine) {
+                    const int c = page_column(view, pos);
+                    page = __ldg(view.table + of.s * view.table_stride + c);
+                    slot = pos - c * view.page_size;
+                }
+            };
+            find(g, g.begin);
+            for (bool more = true; more && ok;) {
+                Segment following;
+                more = plan.next(g, following);
+                for (int t = g.begin; t < g.end; ++t) {
+                    if (!slot_empty()) break;
+                    const uint32_t s = used % kSlots;
+                    const int count = __popc(__ballot_sync(0xffffffffu, mine));
+                    if (lane == 0) mbar_arrive_expect_tx(&s_full[s], static_cast<uint32_t>(count) * box_bytes);
+                    __syncwarp();
+                    if (mine) load_box(smem + s * kSlotBytes + at, which == 0 ? &map_k : &map_v, column * 64, slot, g.head, page, &s_full[s]);
+                    ++used;
+                    // The next tile's page, looked up while this one is on its way.
+                    if (t + 1 < g.end) {
+                        find(g, t + 1);
+                    } else if (more) {
+                        find(following, following.begin);
+                    }
+                }
+                if (!ok || !slot_empty()) break;
+                if (lane == 0) mbar_arrive_cta(&s_full[used % kSlots]);  // empty: the warps' joining buffer
+                ++used;
+                g = following;
+            }
+            if (*abort_flag) {
+                // Copies in flight land before the CTA retires.
+                for (uint32_t i = used > kSlots ? used - kSlots : 0; i < used; ++i) {
+                    mbar_wait_bounded(&s_full[i % kSlots], (i / kSlots) & 1u, p.status, kStatusDrainTimeout);
+                }
+            }
+        } else {
+            constexpr int kPieces = DP / 8;  // 16-byte pieces of a row
+            constexpr int kRowsPerStep = 32 * stream_producers<TMA>() / kPieces;
+            const int id = tid - 32 * kStreamWarps;
+            const int piece = id % kPieces, row0 = id / kPieces;
+            const bool inside = piece * 8 < view.head_dim;
+            for (bool more = true; more && ok;) {
+                const uint8_t* keys = view.keys + 2 * g.head * view.head_stride;
+                const uint8_t* values = view.values + 2 * g.head * view.head_stride;
+                for (int t = g.begin; t < g.end; ++t) {
+                    if (!slot_empty()) break;
+                    const uint32_t s = used % kSlots;
+                    const uint32_t dst = smem + s * kSlotBytes + (piece >> 3) * kColumnBytes;
+#pragma unroll
+                    for (int row = row0; row < kStreamKeys; row += kRowsPerStep) {
+                        const int pos = (g.range.first + t) * kStreamKeys + row;
+                        const long long from = pos >= g.range.lo && pos < g.range.hi ? slot_offset(view, g.s, pos) : -1;
+                        const bool valid = from >= 0 && inside;
+                        const long long at = valid ? 2 * (from + piece * 8) : 0;
+                        const uint32_t to = dst + row * 128 + (((piece & 7) ^ (row & 7)) << 4);
+                        cp_async16(to, keys + at, valid);
+                        cp_async16(to + kColumns * kColumnBytes, values + at, valid);
+                    }
+                    cp_async_arrive(&s_full[s]);
+                    ++used;
+                }
+                if (!ok || !slot_empty()) break;
+                mbar_arrive_cta(&s_full[used % kSlots]);  // empty: the warps' joining buffer
+                ++used;
+                Segment following;
+                more = plan.next(g, following);
+                g = following;
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+        }
+        return;
+    }
 
-    for (;;) {
+    // ---------------- computing warps ----------------
+    const int wr = warp % WM, wk = warp / WM;
+    const int key0 = wk * KW;
+    uint32_t used = 0;  // slots taken
+    for (bool more = true; more;) {
         const int rows = g.seq.n * p.group;
         const int cap = static_cast<int>(min(static_cast<long long>(g.seq.length), static_cast<long long>(view.table_cols) * view.page_size));
-        const uint8_t* kbase = view.keys + 2 * g.head * view.head_stride;
-        const uint8_t* vbase = view.values + 2 * g.head * view.head_stride;
-
-        // Slots of this thread's rows of a tile, found one tile ahead of their copies.
-        long long slots[kSteps];
-        auto find = [&](int tile) {
-#pragma unroll
-            for (int i = 0; i < kSteps; ++i) {
-                const int pos = (g.range.first + tile) * kStreamKeys + my_row + i * kRowsPerStep;
-                slots[i] = pos >= g.range.lo && pos < g.range.hi ? slot_offset(view, g.s, pos) : -1;
-            }
-        };
-        auto copy = [&](int stage) {
-            const uint32_t dst = smem_base + stage * stream_stage_bytes<DP>();
-#pragma unroll
-            for (int i = 0; i < kSteps; ++i) {
-                const int row = my_row + i * kRowsPerStep;
-                const bool valid = slots[i] >= 0 && my_piece_valid;
-                const long long at = valid ? 2 * (slots[i] + my_piece * 8) : 0;
-                const uint32_t off = static_cast<uint32_t>(row * DP * 2 + ((my_piece ^ (row & 7)) << 4));
-                cp_async16(dst + off, kbase + at, valid);
-                cp_async16(dst + kStreamKeys * DP * 2 + off, vbase + at, valid);
-            }
-        };
-
-        const int tiles = g.end - g.begin;
-        find(g.begin);
-#pragma unroll
-        for (int i = 0; i < kStages - 1; ++i) {
-            if (i < tiles) {
-                copy(i);
-                if (i + 1 < tiles) find(g.begin + i + 1);
-            }
-            cp_async_commit();
-        }
 
         // Queries, as the first product's left fragments: rows lane / 4 and lane / 4 + 8 of the
         // warp's 16, elements 2 (lane % 4) + {0, 1} and + 8 of each 16.
@@ -190,24 +305,16 @@ __global__ void __launch_bounds__(kStreamThreads, stream_ctas_per_sm<DP>()) stre
             for (int j = 0; j < 4; ++j) o[i][j] = 0.0f;
         }
         float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
+        bool ok = true;
 
-        int stage = 0;
 #pragma unroll 1
-        for (int t = 0; t < tiles; ++t) {
-            cp_async_wait<kStages - 2>();
-            __syncthreads();
-            {
-                int ahead = stage + kStages - 1;
-                if (ahead >= kStages) ahead -= kStages;
-                if (t + kStages - 1 < tiles) {
-                    copy(ahead);
-                    if (t + kStages < tiles) find(g.begin + t + kStages);
-                }
-                cp_async_commit();
-            }
-            const uint32_t kt = smem_base + stage * stream_stage_bytes<DP>();
-            const uint32_t vt = kt + kStreamKeys * DP * 2;
-            const int key0 = wk * KW;
+        for (int t = g.begin; t < g.end && ok; ++t, ++used) {
+            const uint32_t slot = used % kSlots;
+            ok = __all_sync(0xffffffffu, wait(&s_full[slot], (used / kSlots) & 1u));
+            if (!ok) break;
+            const uint32_t kt = smem + slot * kSlotBytes;
+            const uint32_t vt = kt + kColumns * kColumnBytes;
+            const int pos0 = (g.range.first + t) * kStreamKeys;
 
             float s[KW / 8][4];
 #pragma unroll
@@ -217,19 +324,33 @@ __global__ void __launch_bounds__(kStreamThreads, stream_ctas_per_sm<DP>()) stre
             }
 #pragma unroll
             for (int n = 0; n < KW / 16; ++n) {
+                const int row = key0 + n * 16 + (lane & 7) + ((lane >> 4) << 3);
 #pragma unroll
                 for (int kk = 0; kk < DP / 16; ++kk) {
                     uint32_t b[4];
-                    const int row = key0 + n * 16 + (lane & 7) + ((lane >> 4) << 3);
                     const int piece = kk * 2 + ((lane >> 3) & 1);
-                    ldmatrix4(b, kt + row * DP * 2 + ((piece ^ (row & 7)) << 4));
+                    ldmatrix4(b, kt + (kk >> 2) * kColumnBytes + row * 128 + (((piece & 7) ^ (row & 7)) << 4));
                     mma16816<T>(s[2 * n], qf[kk], b[0], b[1]);
                     mma16816<T>(s[2 * n + 1], qf[kk], b[2], b[3]);
                 }
             }
 
-            const int pos0 = (g.range.first + g.begin + t) * kStreamKeys;
             const bool whole = pos0 >= all_lo && pos0 + kStreamKeys <= all_hi;
+            bool cleared = false;
+            if constexpr (TMA) {
+                const int a = g.range.lo - pos0, b = g.range.hi - pos0;  // rows of the tile that are the unit's keys
+                if (a > key0 || b < key0 + KW) {
+                    for (int i = lane; i < KW * 8 * kColumns; i += 32) {
+                        const int row = key0 + (i >> 3) % KW;
+                        if (row < a || row >= b) {
+                            const uint32_t at = vt + (i >> 3) / KW * kColumnBytes + row * 128 + (i & 7) * 16;
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
+                        }
+                    }
+                    __syncwarp();
+                    cleared = true;
+                }
+            }
             float best[2] = {-INFINITY, -INFINITY};
 #pragma unroll
             for (int n = 0; n < KW / 8; ++n) {
@@ -276,43 +397,50 @@ __global__ void __launch_bounds__(kStreamThreads, stream_ctas_per_sm<DP>()) stre
             for (int n = 0; n < KW / 16; ++n) {
                 const uint32_t a[4] = {pack2<T>(s[2 * n][0], s[2 * n][1]), pack2<T>(s[2 * n][2], s[2 * n][3]),
                                        pack2<T>(s[2 * n + 1][0], s[2 * n + 1][1]), pack2<T>(s[2 * n + 1][2], s[2 * n + 1][3])};
+                const int row = key0 + n * 16 + (lane & 15);
 #pragma unroll
                 for (int i = 0; i < DP / 16; ++i) {
                     uint32_t b[4];
-                    const int row = key0 + n * 16 + (lane & 15);
                     const int piece = i * 2 + (lane >> 4);
-                    ldmatrix4_trans(b, vt + row * DP * 2 + ((piece ^ (row & 7)) << 4));
+                    ldmatrix4_trans(b, vt + (i >> 2) * kColumnBytes + row * 128 + (((piece & 7) ^ (row & 7)) << 4));
                     mma16816<T>(o[2 * i], a, b[0], b[1]);
                     mma16816<T>(o[2 * i + 1], a, b[2], b[3]);
                 }
             }
-            if (++stage == kStages) stage = 0;
+            if (cleared) fence_proxy_async_shared();  // before the slot is loaded into again
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cta(&s_empty[slot]);
         }
 
         // Join the warps that shared the rows, and write the unit's rows or its partial result.
-        cp_async_wait<0>();
-        __syncthreads();
-        float* buffer = reinterpret_cast<float*>(smem);  // [WK][R][kLine]
+        const uint32_t slot = used % kSlots;
+        ok = ok && __all_sync(0xffffffffu, wait(&s_full[slot], (used / kSlots) & 1u));
+        ++used;
+        // [WK][R][DP], elements permuted by 8 with the row so that the stores spread over the banks.
+        float* buffer = reinterpret_cast<float*>(smem_raw + (smem - smem_u32(smem_raw)) + slot * kSlotBytes);
+        if (ok) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
-            sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
-            const int r = wr * 16 + (lane >> 2) + 8 * h;
-            if ((lane & 3) == 0) {
-                s_ml[wk][r][0] = top[h];
-                s_ml[wk][r][1] = sum[h];
-            }
+            for (int h = 0; h < 2; ++h) {
+                sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
+                sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
+                const int r = wr * 16 + (lane >> 2) + 8 * h;
+                if ((lane & 3) == 0) {
+                    s_ml[wk][r][0] = top[h];
+                    s_ml[wk][r][1] = sum[h];
+                }
 #pragma unroll
-            for (int i = 0; i < DP / 8; ++i) {
-                *reinterpret_cast<float2*>(buffer + (wk * R + r) * kLine + i * 8 + 2 * (lane & 3)) = make_float2(o[i][2 * h], o[i][2 * h + 1]);
+                for (int i = 0; i < DP / 8; ++i) {
+                    *reinterpret_cast<float2*>(buffer + (wk * R + r) * DP + ((i * 8 + 2 * (lane & 3)) ^ ((r & 3) << 3))) =
+                        make_float2(o[i][2 * h], o[i][2 * h + 1]);
+                }
             }
         }
-        __syncthreads();
+        ok = stream_barrier(ok);
+        if (!ok) break;
         const bool whole_unit = g.begin == 0 && g.end == g.range.count;
         const int live_rows = min(R, rows - g.rt * R);
-        const long long cta = blockIdx.x;
-        const long long slot = plan.slot(cta, g.unit_start);
-        for (int i = tid; i < live_rows * (DP / 4); i += kStreamThreads) {
+        const long long part = plan.slot(blockIdx.x, g.unit_start);
+        for (int i = tid; i < live_rows * (DP / 4); i += 32 * kStreamWarps) {
             const int r = i / (DP / 4), d = (i % (DP / 4)) * 4;
             float m = s_ml[0][r][0];
 #pragma unroll
@@ -323,12 +451,12 @@ __global__ void __launch_bounds__(kStreamThreads, stream_ctas_per_sm<DP>()) stre
 #pragma unroll
             for (int w = 0; w < WK; ++w) {
                 const float f = exp2_approx(s_ml[w][r][0] - base);
-                const float4 part = *reinterpret_cast<const float4*>(buffer + (w * R + r) * kLine + d);
+                const float4 of = *reinterpret_cast<const float4*>(buffer + (w * R + r) * DP + (d ^ ((r & 3) << 3)));
                 l += f * s_ml[w][r][1];
-                y.x += f * part.x;
-                y.y += f * part.y;
-                y.z += f * part.z;
-                y.w += f * part.w;
+                y.x += f * of.x;
+                y.y += f * of.y;
+                y.z += f * of.z;
+                y.w += f * of.w;
             }
             if (whole_unit) {
                 const int row = g.rt * R + r;
@@ -344,26 +472,28 @@ __global__ void __launch_bounds__(kStreamThreads, stream_ctas_per_sm<DP>()) stre
                     p.lse[token * p.q_heads + head] = l > 0.0f ? (base + log2f(l)) * 0.69314718056f : (l == 0.0f ? -INFINITY : l);
                 }
             } else {
-                *reinterpret_cast<float4*>(p.part_o + (slot * R + r) * DP + d) = y;
-                if (d == 0) *reinterpret_cast<float2*>(p.part_ml + (slot * R + r) * 2) = make_float2(m, l);
+                *reinterpret_cast<float4*>(p.part_o + (part * R + r) * DP + d) = y;
+                if (d == 0) *reinterpret_cast<float2*>(p.part_ml + (part * R + r) * 2) = make_float2(m, l);
             }
         }
+        if (!whole_unit) __threadfence();
+        fence_proxy_async_shared();  // before the slot is loaded into again
+        stream_barrier(true);        // every warp is done with the buffer and with s_ml
+        if (lane == 0) mbar_arrive_cta(&s_empty[slot]);
         if (!whole_unit) {
-            __threadfence();
-            __syncthreads();
             if (tid == 0) {
                 const long long c_first = g.unit_start / plan.quota, c_last = (g.unit_start + g.range.count - 1) / plan.quota;
                 s_last = arrive_last(p.tickets + c_first, p.epoch, static_cast<uint32_t>(c_last - c_first + 1)) ? 1 : 0;
             }
-            __syncthreads();
+            stream_barrier(true);
             if (s_last) {
                 __threadfence();
-                join_partials<T, R, DP, kStreamThreads>(p, plan, g);
+                join_partials<T, R, DP, 32 * kStreamWarps>(p, plan, g);
             }
+            stream_barrier(true);  // s_last is read before it is written again
         }
-        __syncthreads();  // the buffer is free again
         Segment following;
-        if (!plan.next(g, following)) break;
+        more = plan.next(g, following);
         g = following;
     }
 }
