@@ -292,25 +292,33 @@ struct Planner {
     }
 };
 
-// Counts the arrivals at one ticket; true for the last of `expected`, which leaves it at zero.
+// Counts the arrivals at one ticket; true for the last of `expected`, which leaves it at zero. An
+// addition is enough where the ticket already is of this epoch; whoever finds another one there (its
+// addition to that does not count) sets it, or adds again where somebody else just did.
 __device__ __forceinline__ bool arrive_last(u64* ticket, uint32_t epoch, uint32_t expected) {
-    u64 seen = *reinterpret_cast<volatile u64*>(ticket);
-    for (;;) {
-        const uint32_t count = (seen >> 32) == epoch ? static_cast<uint32_t>(seen) + 1u : 1u;
-        const u64 next = count >= expected ? 0ull : (static_cast<u64>(epoch) << 32) | count;
-        const u64 old = atomicCAS(ticket, seen, next);
-        if (old == seen) return count >= expected;
-        seen = old;
+    u64 seen = atomicAdd(ticket, 1ull);
+    while ((seen >> 32) != epoch) {
+        const u64 mine = (static_cast<u64>(epoch) << 32) | 1ull;
+        const u64 now = *reinterpret_cast<volatile u64*>(ticket);
+        if ((now >> 32) == epoch) {
+            seen = atomicAdd(ticket, 1ull);
+        } else if (atomicCAS(ticket, now, mine) == now) {
+            seen = mine - 1ull;
+        }
     }
+    const bool last = static_cast<uint32_t>(seen) + 1u == expected;
+    if (last) *reinterpret_cast<volatile u64*>(ticket) = 0ull;
+    return last;
 }
 
 // Joins the partial results of a cut unit and writes its rows' output. Every thread of the CTA
-// that arrived last calls it (THREADS of them, by tid). A warp takes 4 rows at a time, so that
-// their loads are in flight together; its lanes first hold the maxima and sums of up to 32 CTAs
+// that arrived last calls it (THREADS of them, by tid). A warp takes some rows at a time, so
+// that their loads are in flight together; its lanes first hold the maxima and sums of up to 32 CTAs
 // each, then DP / 32 elements of the rows. The sums run in the order of the CTAs.
 template <typename T, int R, int DP, int THREADS, typename PLAN>
 __device__ void join_partials(const AttnParams& p, const PLAN& plan, const Segment& g) {
-    constexpr int kRows = 4, kWarps = THREADS / 32, kPer = DP / 32;
+    // Decoding has few rows and many parts, longer chunks the other way round: 16 loads in flight.
+    constexpr int kRows = R == 16 ? 2 : 4, kUnroll = 16 / kRows, kWarps = THREADS / 32, kPer = DP / 32;
     const int rows = min(R, g.seq.n * p.group - g.rt * R);
     const long long c_first = g.unit_start / plan.quota;
     const int parts = static_cast<int>((g.unit_start + g.range.count - 1) / plan.quota - c_first) + 1;
@@ -346,7 +354,7 @@ __device__ void join_partials(const AttnParams& p, const PLAN& plan, const Segme
                 l[u] = w[u] * ml.y;
             }
             const int n = min(32, parts - c0);
-#pragma unroll 2
+#pragma unroll kUnroll
             for (int c = 0; c < n; ++c) {
 #pragma unroll
                 for (int u = 0; u < kRows; ++u) {
