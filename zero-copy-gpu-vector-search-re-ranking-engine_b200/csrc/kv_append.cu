@@ -9,9 +9,12 @@
 // 16 bytes each, so all loads and stores are 16 bytes wide and a head's sum of squares is three or
 // four shuffles. A pair of the split form lies rotary_dim / 16 lanes apart (rotary_dim is a
 // multiple of 16), so it is exchanged by shuffles too; a pair of the interleaved form lies within
-// a lane. One block takes one token (the cosines and sines are then loaded once for all its
-// heads); its first warp finds the token's sequence, position and slot while the values' loads,
-// which do not depend on them, are in flight.
+// a lane. A block takes up to 8 tokens, one after the other: its warps find a token's sequence,
+// position and slot each while the first values are on their way, and every token's values and
+// cosines are loaded while the one before is worked on. (A token per block left the search, the
+// rotation row and the stores one behind the other: 18,293 tokens of 48 heads took 163 us.)
+#include <algorithm>
+
 #include "common.cuh"
 #include "paged.h"
 
@@ -22,6 +25,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kHeadsPerLane = 4;  // loads in flight per thread
+constexpr int kMaxTokens = kThreads / 32;  // of a block: a warp finds the place of each
 
 struct AppendParams {
     View view;
@@ -42,6 +46,7 @@ struct AppendParams {
     int q_heads;
     int heads;   // of all three: q_heads + 2 * kv_heads, without the ones not given
     int chunks;  // blocks per token
+    int tokens_per_block;
 };
 
 // Number of entries of starts[1 .. sequences] that are <= token: the token's sequence, or
@@ -59,146 +64,173 @@ __device__ __forceinline__ int sequence_of(const View& v, int token, int lane) {
     return lo;
 }
 
+// Where a token goes.
+struct Place {
+    long long slot;  // element offset in keys and values; -1: not stored
+    int row;         // rotation row; -1: outside the table, -2: a padding token
+};
+
 template <typename T, int LANES>
-__global__ void __launch_bounds__(kThreads) append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(kThreads, 2) append_kernel(const AppendParams p) {
     constexpr int kSegments = kThreads / LANES;
-    __shared__ long long s_slot;
-    __shared__ int s_row;  // rotation row; -1: outside the table, -2: a padding token
+    __shared__ Place s_place[kMaxTokens];
     const View& view = p.view;
     const int tid = threadIdx.x;
     const int lane = tid & (LANES - 1);
     const int segment = tid / LANES;
-    const int token = static_cast<int>(blockIdx.x / static_cast<unsigned>(p.chunks));
+    const int token0 = static_cast<int>(blockIdx.x / static_cast<unsigned>(p.chunks)) * p.tokens_per_block;
+    const int tokens = min(p.tokens_per_block, view.tokens - token0);
     const int first = static_cast<int>(blockIdx.x % static_cast<unsigned>(p.chunks)) * kSegments * kHeadsPerLane + segment;
     const bool holds = lane * 8 < view.head_dim;
     const int k_begin = p.q_heads;
     const int v_begin = p.q_heads + (p.k != nullptr ? view.kv_heads : 0);
 
-    uint4 x[kHeadsPerLane];
+    // This thread's pieces of a token's heads.
+    auto load = [&](int token, uint4 (&x)[kHeadsPerLane]) {
 #pragma unroll
-    for (int u = 0; u < kHeadsPerLane; ++u) {
-        const int h = first + u * kSegments;
-        x[u] = make_uint4(0u, 0u, 0u, 0u);
-        if (h >= p.heads || !holds) continue;
-        const uint8_t* base;
-        long long at;
-        if (h < k_begin) {
-            base = p.q;
-            at = token * p.q_token + h * p.q_head;
-        } else if (h < v_begin) {
-            base = p.k;
-            at = token * p.k_token + (h - k_begin) * p.k_head;
-        } else {
-            base = p.v;
-            at = token * p.v_token + (h - v_begin) * p.v_head;
+        for (int u = 0; u < kHeadsPerLane; ++u) {
+            const int h = first + u * kSegments;
+            x[u] = make_uint4(0u, 0u, 0u, 0u);
+            if (h >= p.heads || !holds) continue;
+            const uint8_t* base;
+            long long at;
+            if (h < k_begin) {
+                base = p.q;
+                at = token * p.q_token + h * p.q_head;
+            } else if (h < v_begin) {
+                base = p.k;
+                at = token * p.k_token + (h - k_begin) * p.k_head;
+            } else {
+                base = p.v;
+                at = token * p.v_token + (h - v_begin) * p.v_head;
+            }
+            x[u] = *reinterpret_cast<const uint4*>(base + 2 * (at + lane * 8));
         }
-        x[u] = *reinterpret_cast<const uint4*>(base + 2 * (at + lane * 8));
-    }
+    };
+    // This lane's cosines and sines: of its 8 elements, or of its 4 pairs in the interleaved form.
+    const int half = p.rotary_dim / 2;
+    const bool turns = p.rotary != nullptr && lane * 8 < p.rotary_dim;
+    const int in_row = p.interleaved ? lane * 4 : (lane * 8) % half;
+    auto load_turn = [&](int row, float4 (&cs)[2], float4 (&sn)[2]) {
+        if (!turns || row < 0) return;
+        const float* c = p.rotary + static_cast<long long>(row) * p.rotary_dim + in_row;
+        cs[0] = __ldg(reinterpret_cast<const float4*>(c));
+        sn[0] = __ldg(reinterpret_cast<const float4*>(c + half));
+        if (!p.interleaved) {
+            cs[1] = __ldg(reinterpret_cast<const float4*>(c + 4));
+            sn[1] = __ldg(reinterpret_cast<const float4*>(c + half + 4));
+        }
+    };
 
-    if (tid < 32) {
-        const int s = sequence_of(view, token, tid);
-        if (tid == 0) {
-            long long slot = -1;
-            int row = -2;
+    uint4 x[kHeadsPerLane];
+    load(token0, x);
+    if (tid / 32 < tokens) {
+        const int token = token0 + tid / 32;
+        const int s = sequence_of(view, token, tid & 31);
+        if ((tid & 31) == 0) {
+            Place place{-1, -2};
             if (s < view.sequences) {
                 const long long end = view.starts[s + 1];
                 const long long at = view.lengths[s] - end + token;  // negative: not among the cached ones
                 const int position = static_cast<int>(max(at, -1LL));
                 const long long turn = p.positions != nullptr ? p.positions[token] : at;
-                row = 0;
-                if (p.rotary != nullptr) row = turn >= 0 && turn < p.rotary_rows ? static_cast<int>(turn) : -1;
-                if (p.k != nullptr) slot = slot_offset(view, s, position);
+                place.row = 0;
+                if (p.rotary != nullptr) place.row = turn >= 0 && turn < p.rotary_rows ? static_cast<int>(turn) : -1;
+                if (p.k != nullptr && place.row >= 0) place.slot = slot_offset(view, s, position);
             }
-            s_slot = slot;
-            s_row = row;
+            s_place[tid / 32] = place;
         }
     }
     __syncthreads();
-    const int row = s_row;
-    if (row == -2) return;
-    const long long slot = row >= 0 ? s_slot : -1;
-
-    // This lane's cosines and sines: of its 8 elements, or of its 4 pairs in the interleaved form.
-    const int half = p.rotary_dim / 2;
-    const bool turned = p.rotary != nullptr && row >= 0 && lane * 8 < p.rotary_dim;
-    float cs[8], sn[8];
-    if (turned) {
-        const float* c = p.rotary + static_cast<long long>(row) * p.rotary_dim + (p.interleaved ? lane * 4 : (lane * 8) % half);
-        const float4 c0 = __ldg(reinterpret_cast<const float4*>(c)), s0 = __ldg(reinterpret_cast<const float4*>(c + half));
-        cs[0] = c0.x; cs[1] = c0.y; cs[2] = c0.z; cs[3] = c0.w;
-        sn[0] = s0.x; sn[1] = s0.y; sn[2] = s0.z; sn[3] = s0.w;
-        if (!p.interleaved) {
-            const float4 c1 = __ldg(reinterpret_cast<const float4*>(c + 4)), s1 = __ldg(reinterpret_cast<const float4*>(c + half + 4));
-            cs[4] = c1.x; cs[5] = c1.y; cs[6] = c1.z; cs[7] = c1.w;
-            sn[4] = s1.x; sn[5] = s1.y; sn[6] = s1.z; sn[7] = s1.w;
-            if (lane * 8 < half) {  // a cos - b sin; the other half is b cos + a sin
-#pragma unroll
-                for (int i = 0; i < 8; ++i) sn[i] = -sn[i];
-            }
-        }
-    }
-    // The lane that holds the other element of this lane's pairs (split form).
+    float4 cs[2] = {}, sn[2] = {};
+    load_turn(s_place[0].row, cs, sn);
+    // The lane that holds the other element of this lane's pairs (split form), and the sign of its
+    // part: a cos - b sin, b cos + a sin.
     const int apart = half / 8;
-    const int partner = lane < apart ? lane + apart : lane - apart;
+    const int partner = (lane < apart ? lane + apart : lane - apart) & (LANES - 1);
+    const float sign = lane < apart ? -1.0f : 1.0f;
 
-#pragma unroll
-    for (int u = 0; u < kHeadsPerLane; ++u) {
-        const int h = first + u * kSegments;
-        if (first - segment + u * kSegments >= p.heads) break;  // for the whole block, so that the shuffles see every lane
-        const uint8_t* weight = h < k_begin ? p.q_norm : p.k_norm;
-        const bool is_value = h >= v_begin;
-        float f[8];
-        const uint32_t packed[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 t = unpack2<T>(packed[i]);
-            f[2 * i] = t.x;
-            f[2 * i + 1] = t.y;
+#pragma unroll 1
+    for (int i = 0; i < tokens; ++i) {
+        const int token = token0 + i;
+        const Place place = s_place[i];
+        uint4 ahead[kHeadsPerLane];
+        float4 cs_ahead[2] = {}, sn_ahead[2] = {};
+        if (i + 1 < tokens) {
+            load(token + 1, ahead);
+            load_turn(s_place[i + 1].row, cs_ahead, sn_ahead);
         }
-        float sum = 0.0f;
+        if (place.row != -2) {
+            const bool turned = turns && place.row >= 0;
+            const float c8[8] = {cs[0].x, cs[0].y, cs[0].z, cs[0].w, cs[1].x, cs[1].y, cs[1].z, cs[1].w};
+            const float s8[8] = {sn[0].x, sn[0].y, sn[0].z, sn[0].w, sn[1].x, sn[1].y, sn[1].z, sn[1].w};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum += f[i] * f[i];
+            for (int u = 0; u < kHeadsPerLane; ++u) {
+                const int h = first + u * kSegments;
+                if (first - segment + u * kSegments >= p.heads) break;  // for the whole block, so that the shuffles see every lane
+                const uint8_t* weight = h < k_begin ? p.q_norm : p.k_norm;
+                const bool is_value = h >= v_begin;
+                float f[8];
+                const uint32_t packed[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
 #pragma unroll
-        for (int o = LANES / 2; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o, LANES);
-        if (!is_value && weight != nullptr && holds) {
-            const float inv = rsqrtf(sum / static_cast<float>(view.head_dim) + p.eps);
-            const uint4 w = __ldg(reinterpret_cast<const uint4*>(weight) + lane);
-            const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+                for (int j = 0; j < 4; ++j) {
+                    const float2 t = unpack2<T>(packed[j]);
+                    f[2 * j] = t.x;
+                    f[2 * j + 1] = t.y;
+                }
+                float sum = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float2 t = unpack2<T>(ws[i]);
-                f[2 * i] *= inv * t.x;
-                f[2 * i + 1] *= inv * t.y;
-            }
-        }
-        if (p.rotary != nullptr) {
-            if (p.interleaved) {
-                if (turned && !is_value) {
+                for (int j = 0; j < 8; ++j) sum += f[j] * f[j];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float a = f[2 * i], b = f[2 * i + 1];
-                        f[2 * i] = a * cs[i] - b * sn[i];
-                        f[2 * i + 1] = b * cs[i] + a * sn[i];
+                for (int o = LANES / 2; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o, LANES);
+                if (!is_value && weight != nullptr && holds) {
+                    const float inv = rsqrtf(sum / static_cast<float>(view.head_dim) + p.eps);
+                    const uint4 w = __ldg(reinterpret_cast<const uint4*>(weight) + lane);
+                    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float2 t = unpack2<T>(ws[j]);
+                        f[2 * j] *= inv * t.x;
+                        f[2 * j + 1] *= inv * t.y;
                     }
                 }
-            } else {
+                if (p.rotary != nullptr) {
+                    if (p.interleaved) {
+                        if (turned && !is_value) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float other = __shfl_sync(0xffffffffu, f[i], partner & (LANES - 1), LANES);
-                    if (turned && !is_value) f[i] = f[i] * cs[i] + other * sn[i];
+                            for (int j = 0; j < 4; ++j) {
+                                const float a = f[2 * j], b = f[2 * j + 1];
+                                f[2 * j] = a * c8[j] - b * s8[j];
+                                f[2 * j + 1] = b * c8[j] + a * s8[j];
+                            }
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const float other = __shfl_sync(0xffffffffu, f[j], partner, LANES);
+                            if (turned && !is_value) f[j] = f[j] * c8[j] + sign * other * s8[j];
+                        }
+                    }
+                }
+                uint4 y = make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
+                if (is_value) y = x[u];  // bit for bit, NaN payloads included
+                if (h >= p.heads || !holds) continue;
+                if (h < k_begin) {
+                    if (place.row < 0) y = make_uint4(0u, 0u, 0u, 0u);
+                    *reinterpret_cast<uint4*>(p.q_out + 2 * (token * p.q_out_token + h * p.q_out_head + lane * 8)) = y;
+                } else if (place.slot >= 0) {
+                    const int head = is_value ? h - v_begin : h - k_begin;
+                    uint8_t* base = is_value ? view.values : view.keys;
+                    *reinterpret_cast<uint4*>(base + 2 * (place.slot + head * view.head_stride + lane * 8)) = y;
                 }
             }
         }
-        uint4 y = make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
-        if (is_value) y = x[u];  // bit for bit, NaN payloads included
-        if (h >= p.heads || !holds) continue;
-        if (h < k_begin) {
-            if (row < 0) y = make_uint4(0u, 0u, 0u, 0u);
-            *reinterpret_cast<uint4*>(p.q_out + 2 * (token * p.q_out_token + h * p.q_out_head + lane * 8)) = y;
-        } else if (slot >= 0) {
-            const int head = is_value ? h - v_begin : h - k_begin;
-            uint8_t* base = is_value ? view.values : view.keys;
-            *reinterpret_cast<uint4*>(base + 2 * (slot + head * view.head_stride + lane * 8)) = y;
+#pragma unroll
+        for (int u = 0; u < kHeadsPerLane; ++u) x[u] = ahead[u];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            cs[j] = cs_ahead[j];
+            sn[j] = sn_ahead[j];
         }
     }
 }
@@ -287,7 +319,10 @@ extern "C" int zcgvs_kv_append(const zcgvs_paged_cache* cache, const zcgvs_step_
     p.q_heads = q_heads;
     p.heads = static_cast<int>(heads);
     p.chunks = static_cast<int>(chunks);
-    const unsigned blocks = static_cast<unsigned>(chunks * batch->tokens);
+    // Enough blocks to fill the SMs twice over come first, then more tokens per block.
+    const long long fill = 4LL * device_sm_count();
+    p.tokens_per_block = static_cast<int>(std::min<long long>(std::max<long long>(chunks * batch->tokens / fill, 1), kMaxTokens));
+    const unsigned blocks = static_cast<unsigned>(chunks * ((batch->tokens + p.tokens_per_block - 1) / p.tokens_per_block));
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const cudaError_t e = cache->dtype == ZCGVS_DTYPE_F16 ? launch_append<__half>(p, blocks, narrow, s)
                                                           : launch_append<__nv_bfloat16>(p, blocks, narrow, s);
