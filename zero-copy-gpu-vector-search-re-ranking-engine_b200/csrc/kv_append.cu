@@ -5,14 +5,16 @@
 //   (a, b) -> (a cos - b sin, b cos + a sin)          (pairs of the first rotary_dim elements)
 //
 // Bound by memory: every value is read once and written once, 2 * 2 bytes per value, and the
-// rotation table's row once per token. A head's row is held by 8 lanes (head_dim <= 64) or 16,
-// 16 bytes each, so all loads and stores are 16 bytes wide and a head's sum of squares is three or
-// four shuffles. A pair of the split form lies rotary_dim / 16 lanes apart (rotary_dim is a
-// multiple of 16), so it is exchanged by shuffles too; a pair of the interleaved form lies within
-// a lane. A block takes up to 8 tokens, one after the other: its warps find a token's sequence,
-// position and slot each while the first values are on their way, and every token's values and
-// cosines are loaded while the one before is worked on. (A token per block left the search, the
-// rotation row and the stores one behind the other: 18,293 tokens of 48 heads took 163 us.)
+// rotation table's row once per token; next by the instructions per head. A head's row is held by 8
+// lanes (head_dim <= 64) or 16, 8 elements each: 4 of the first and 4 of the second half of the
+// rotated elements (or 8 neighbours, in the interleaved form and past the rotated ones), so that both
+// elements of a pair are in one lane and only the sum of squares goes through shuffles. (16-byte
+// pieces, with the pairs exchanged by shuffles, took 236 instructions per head, and that was the
+// bound: 18,293 tokens of 48 heads in 140 us.)
+//
+// A block takes up to 8 tokens, one after the other: its warps find a token's sequence, position and
+// slot each while the first values are on their way, and every token's values and cosines are
+// loaded while the one before is worked on.
 #include <algorithm>
 
 #include "common.cuh"
@@ -85,45 +87,66 @@ __global__ void __launch_bounds__(kThreads, 2) append_kernel(const AppendParams 
     const int k_begin = p.q_heads;
     const int v_begin = p.q_heads + (p.k != nullptr ? view.kv_heads : 0);
 
-    // This thread's pieces of a token's heads.
-    auto load = [&](int token, uint4 (&x)[kHeadsPerLane]) {
+    // This lane's elements: 4 from `at0` and 4 from `at1`.
+    const bool turns = p.rotary != nullptr && lane * 8 < p.rotary_dim;
+    const int half = p.rotary_dim / 2;
+    const bool apart = turns && !p.interleaved;
+    const int at0 = apart ? lane * 4 : lane * 8;
+    const int at1 = apart ? half + lane * 4 : lane * 8 + 4;
+
+    // Heads are the same for every token: their first token's place and how far apart tokens are.
+    const uint8_t* from[kHeadsPerLane];
+    long long step[kHeadsPerLane];
+    long long to[kHeadsPerLane];  // of a query: its place in q_out (bytes); else the head's in a slot
+#pragma unroll
+    for (int u = 0; u < kHeadsPerLane; ++u) {
+        const int h = first + u * kSegments;
+        const bool key = h >= k_begin && h < v_begin;
+        const int head = h < k_begin ? h : key ? h - k_begin : h - v_begin;
+        const uint8_t* base = h < k_begin ? p.q : key ? p.k : p.v;
+        const long long token_stride = h < k_begin ? p.q_token : key ? p.k_token : p.v_token;
+        const long long head_stride = h < k_begin ? p.q_head : key ? p.k_head : p.v_head;
+        from[u] = base + 2 * (token0 * token_stride + head * head_stride);
+        step[u] = 2 * token_stride;
+        to[u] = 2 * (h < k_begin ? token0 * p.q_out_token + head * p.q_out_head : head * view.head_stride);
+    }
+    auto load = [&](uint2 (&x)[kHeadsPerLane][2]) {
 #pragma unroll
         for (int u = 0; u < kHeadsPerLane; ++u) {
-            const int h = first + u * kSegments;
-            x[u] = make_uint4(0u, 0u, 0u, 0u);
-            if (h >= p.heads || !holds) continue;
-            const uint8_t* base;
-            long long at;
-            if (h < k_begin) {
-                base = p.q;
-                at = token * p.q_token + h * p.q_head;
-            } else if (h < v_begin) {
-                base = p.k;
-                at = token * p.k_token + (h - k_begin) * p.k_head;
-            } else {
-                base = p.v;
-                at = token * p.v_token + (h - v_begin) * p.v_head;
+            x[u][0] = x[u][1] = make_uint2(0u, 0u);
+            if (first + u * kSegments < p.heads && holds) {
+                x[u][0] = *reinterpret_cast<const uint2*>(from[u] + 2 * at0);
+                x[u][1] = *reinterpret_cast<const uint2*>(from[u] + 2 * at1);
             }
-            x[u] = *reinterpret_cast<const uint4*>(base + 2 * (at + lane * 8));
+            from[u] += step[u];
         }
     };
-    // This lane's cosines and sines: of its 8 elements, or of its 4 pairs in the interleaved form.
-    const int half = p.rotary_dim / 2;
-    const bool turns = p.rotary != nullptr && lane * 8 < p.rotary_dim;
-    const int in_row = p.interleaved ? lane * 4 : (lane * 8) % half;
-    auto load_turn = [&](int row, float4 (&cs)[2], float4 (&sn)[2]) {
+    // The cosines and sines of its 4 pairs.
+    auto load_turn = [&](int row, float4& cs, float4& sn) {
         if (!turns || row < 0) return;
-        const float* c = p.rotary + static_cast<long long>(row) * p.rotary_dim + in_row;
-        cs[0] = __ldg(reinterpret_cast<const float4*>(c));
-        sn[0] = __ldg(reinterpret_cast<const float4*>(c + half));
-        if (!p.interleaved) {
-            cs[1] = __ldg(reinterpret_cast<const float4*>(c + 4));
-            sn[1] = __ldg(reinterpret_cast<const float4*>(c + half + 4));
-        }
+        const float* c = p.rotary + static_cast<long long>(row) * p.rotary_dim + lane * 4;
+        cs = __ldg(reinterpret_cast<const float4*>(c));
+        sn = __ldg(reinterpret_cast<const float4*>(c + half));
+    };
+    // Two packed words to two pairs of numbers.
+    auto unpack4 = [](const uint2& v, float2 (&f)[2]) {
+        f[0] = unpack2<T>(v.x);
+        f[1] = unpack2<T>(v.y);
+    };
+    float2 q_weight[4], k_weight[4];
+    auto load_weights = [&](const uint8_t* w, float2 (&f)[4]) {
+        if (w == nullptr || !holds) return;
+        float2 a[2], b[2];
+        unpack4(__ldg(reinterpret_cast<const uint2*>(w + 2 * at0)), a);
+        unpack4(__ldg(reinterpret_cast<const uint2*>(w + 2 * at1)), b);
+        f[0] = a[0];
+        f[1] = a[1];
+        f[2] = b[0];
+        f[3] = b[1];
     };
 
-    uint4 x[kHeadsPerLane];
-    load(token0, x);
+    uint2 x[kHeadsPerLane][2];
+    load(x);
     if (tid / 32 < tokens) {
         const int token = token0 + tid / 32;
         const int s = sequence_of(view, token, tid & 31);
@@ -142,96 +165,100 @@ __global__ void __launch_bounds__(kThreads, 2) append_kernel(const AppendParams 
         }
     }
     __syncthreads();
-    float4 cs[2] = {}, sn[2] = {};
+    float4 cs = {}, sn = {};
     load_turn(s_place[0].row, cs, sn);
-    // The lane that holds the other element of this lane's pairs (split form), and the sign of its
-    // part: a cos - b sin, b cos + a sin.
-    const int apart = half / 8;
-    const int partner = (lane < apart ? lane + apart : lane - apart) & (LANES - 1);
-    const float sign = lane < apart ? -1.0f : 1.0f;
+    load_weights(p.q_norm, q_weight);
+    load_weights(p.k_norm, k_weight);
+    const float per_dim = 1.0f / static_cast<float>(view.head_dim);
 
 #pragma unroll 1
     for (int i = 0; i < tokens; ++i) {
-        const int token = token0 + i;
         const Place place = s_place[i];
-        uint4 ahead[kHeadsPerLane];
-        float4 cs_ahead[2] = {}, sn_ahead[2] = {};
+        uint2 ahead[kHeadsPerLane][2];
+        float4 cs_ahead = {}, sn_ahead = {};
         if (i + 1 < tokens) {
-            load(token + 1, ahead);
+            load(ahead);
             load_turn(s_place[i + 1].row, cs_ahead, sn_ahead);
         }
         if (place.row != -2) {
             const bool turned = turns && place.row >= 0;
-            const float c8[8] = {cs[0].x, cs[0].y, cs[0].z, cs[0].w, cs[1].x, cs[1].y, cs[1].z, cs[1].w};
-            const float s8[8] = {sn[0].x, sn[0].y, sn[0].z, sn[0].w, sn[1].x, sn[1].y, sn[1].z, sn[1].w};
+            const float2 c2[2] = {make_float2(cs.x, cs.y), make_float2(cs.z, cs.w)};
+            const float2 s2[2] = {make_float2(sn.x, sn.y), make_float2(sn.z, sn.w)};
 #pragma unroll
             for (int u = 0; u < kHeadsPerLane; ++u) {
                 const int h = first + u * kSegments;
-                if (first - segment + u * kSegments >= p.heads) break;  // for the whole block, so that the shuffles see every lane
-                const uint8_t* weight = h < k_begin ? p.q_norm : p.k_norm;
                 const bool is_value = h >= v_begin;
-                float f[8];
-                const uint32_t packed[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float2 t = unpack2<T>(packed[j]);
-                    f[2 * j] = t.x;
-                    f[2 * j + 1] = t.y;
-                }
-                float sum = 0.0f;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) sum += f[j] * f[j];
-#pragma unroll
-                for (int o = LANES / 2; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o, LANES);
-                if (!is_value && weight != nullptr && holds) {
-                    const float inv = rsqrtf(sum / static_cast<float>(view.head_dim) + p.eps);
-                    const uint4 w = __ldg(reinterpret_cast<const uint4*>(weight) + lane);
-                    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float2 t = unpack2<T>(ws[j]);
-                        f[2 * j] *= inv * t.x;
-                        f[2 * j + 1] *= inv * t.y;
+                uint2 y[2] = {x[u][0], x[u][1]};  // values bit for bit, NaN payloads included
+                if (__any_sync(0xffffffffu, !is_value)) {
+                    float2 f[4];
+                    {
+                        float2 a[2], b[2];
+                        unpack4(x[u][0], a);
+                        unpack4(x[u][1], b);
+                        f[0] = a[0];
+                        f[1] = a[1];
+                        f[2] = b[0];
+                        f[3] = b[1];
                     }
-                }
-                if (p.rotary != nullptr) {
-                    if (p.interleaved) {
-                        if (turned && !is_value) {
+                    const bool query = h < k_begin;
+                    const bool normed = query ? p.q_norm != nullptr : p.k_norm != nullptr;
+                    if (p.q_norm != nullptr || p.k_norm != nullptr) {
+                        float2 square = both(0.0f);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) square = fma2(f[j], f[j], square);
+                        float sum = square.x + square.y;
+#pragma unroll
+                        for (int o = LANES / 2; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o, LANES);
+                        if (normed) {
+                            const float2 inv = both(rsqrtf(fmaf(sum, per_dim, p.eps)));
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) f[j] = mul2(f[j], mul2(inv, query ? q_weight[j] : k_weight[j]));
+                        }
+                    }
+                    if (turned) {
+                        if (p.interleaved) {
+                            const float c4[4] = {cs.x, cs.y, cs.z, cs.w}, s4[4] = {sn.x, sn.y, sn.z, sn.w};
 #pragma unroll
                             for (int j = 0; j < 4; ++j) {
-                                const float a = f[2 * j], b = f[2 * j + 1];
-                                f[2 * j] = a * c8[j] - b * s8[j];
-                                f[2 * j + 1] = b * c8[j] + a * s8[j];
+                                f[j] = make_float2(f[j].x * c4[j] - f[j].y * s4[j], f[j].y * c4[j] + f[j].x * s4[j]);
+                            }
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 2; ++j) {
+                                const float2 a = f[j], b = f[j + 2];
+                                f[j] = fma2(mul2(b, s2[j]), both(-1.0f), mul2(a, c2[j]));
+                                f[j + 2] = fma2(a, s2[j], mul2(b, c2[j]));
                             }
                         }
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const float other = __shfl_sync(0xffffffffu, f[j], partner, LANES);
-                            if (turned && !is_value) f[j] = f[j] * c8[j] + sign * other * s8[j];
-                        }
+                    }
+                    if (!is_value) {
+                        y[0] = make_uint2(pack2<T>(f[0].x, f[0].y), pack2<T>(f[1].x, f[1].y));
+                        y[1] = make_uint2(pack2<T>(f[2].x, f[2].y), pack2<T>(f[3].x, f[3].y));
                     }
                 }
-                uint4 y = make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
-                if (is_value) y = x[u];  // bit for bit, NaN payloads included
-                if (h >= p.heads || !holds) continue;
-                if (h < k_begin) {
-                    if (place.row < 0) y = make_uint4(0u, 0u, 0u, 0u);
-                    *reinterpret_cast<uint4*>(p.q_out + 2 * (token * p.q_out_token + h * p.q_out_head + lane * 8)) = y;
-                } else if (place.slot >= 0) {
-                    const int head = is_value ? h - v_begin : h - k_begin;
-                    uint8_t* base = is_value ? view.values : view.keys;
-                    *reinterpret_cast<uint4*>(base + 2 * (place.slot + head * view.head_stride + lane * 8)) = y;
+                if (h < p.heads && holds) {
+                    uint8_t* dst;
+                    if (h < k_begin) {
+                        dst = p.q_out + to[u];
+                        if (place.row < 0) y[0] = y[1] = make_uint2(0u, 0u);
+                    } else {
+                        dst = place.slot >= 0 ? (is_value ? view.values : view.keys) + 2 * place.slot + to[u] : nullptr;
+                    }
+                    if (dst != nullptr) {
+                        *reinterpret_cast<uint2*>(dst + 2 * at0) = y[0];
+                        *reinterpret_cast<uint2*>(dst + 2 * at1) = y[1];
+                    }
                 }
             }
         }
 #pragma unroll
-        for (int u = 0; u < kHeadsPerLane; ++u) x[u] = ahead[u];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            cs[j] = cs_ahead[j];
-            sn[j] = sn_ahead[j];
+        for (int u = 0; u < kHeadsPerLane; ++u) {
+            x[u][0] = ahead[u][0];
+            x[u][1] = ahead[u][1];
+            if (first + u * kSegments < k_begin) to[u] += 2 * p.q_out_token;
         }
+        cs = cs_ahead;
+        sn = sn_ahead;
     }
 }
 
