@@ -26,7 +26,7 @@ namespace paged {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kHeadsPerLane = 4;  // loads in flight per thread
+constexpr int kMaxHeads = 4;  // of a token, per lane
 constexpr int kMaxTokens = kThreads / 32;  // of a block: a warp finds the place of each
 
 struct AppendParams {
@@ -72,7 +72,9 @@ struct Place {
     int row;         // rotation row; -1: outside the table, -2: a padding token
 };
 
-template <typename T, int LANES>
+// HEADS heads of a token per lane, no more than needed. (Two blocks per SM with 128 registers: three
+// with 80 are slower, 123 against 97 us for 18,293 tokens of 48 heads, as the loads ahead spill.)
+template <typename T, int LANES, int HEADS>
 __global__ void __launch_bounds__(kThreads, 2) append_kernel(const AppendParams p) {
     constexpr int kSegments = kThreads / LANES;
     __shared__ Place s_place[kMaxTokens];
@@ -82,7 +84,7 @@ __global__ void __launch_bounds__(kThreads, 2) append_kernel(const AppendParams 
     const int segment = tid / LANES;
     const int token0 = static_cast<int>(blockIdx.x / static_cast<unsigned>(p.chunks)) * p.tokens_per_block;
     const int tokens = min(p.tokens_per_block, view.tokens - token0);
-    const int first = static_cast<int>(blockIdx.x % static_cast<unsigned>(p.chunks)) * kSegments * kHeadsPerLane + segment;
+    const int first = static_cast<int>(blockIdx.x % static_cast<unsigned>(p.chunks)) * kSegments * HEADS + segment;
     const bool holds = lane * 8 < view.head_dim;
     const int k_begin = p.q_heads;
     const int v_begin = p.q_heads + (p.k != nullptr ? view.kv_heads : 0);
@@ -95,11 +97,11 @@ __global__ void __launch_bounds__(kThreads, 2) append_kernel(const AppendParams 
     const int at1 = apart ? half + lane * 4 : lane * 8 + 4;
 
     // Heads are the same for every token: their first token's place and how far apart tokens are.
-    const uint8_t* from[kHeadsPerLane];
-    long long step[kHeadsPerLane];
-    long long to[kHeadsPerLane];  // of a query: its place in q_out (bytes); else the head's in a slot
+    const uint8_t* from[HEADS];
+    long long step[HEADS];
+    long long to[HEADS];  // of a query: its place in q_out (bytes); else the head's in a slot
 #pragma unroll
-    for (int u = 0; u < kHeadsPerLane; ++u) {
+    for (int u = 0; u < HEADS; ++u) {
         const int h = first + u * kSegments;
         const bool key = h >= k_begin && h < v_begin;
         const int head = h < k_begin ? h : key ? h - k_begin : h - v_begin;
@@ -110,9 +112,9 @@ __global__ void __launch_bounds__(kThreads, 2) append_kernel(const AppendParams 
         step[u] = 2 * token_stride;
         to[u] = 2 * (h < k_begin ? token0 * p.q_out_token + head * p.q_out_head : head * view.head_stride);
     }
-    auto load = [&](uint2 (&x)[kHeadsPerLane][2]) {
+    auto load = [&](uint2 (&x)[HEADS][2]) {
 #pragma unroll
-        for (int u = 0; u < kHeadsPerLane; ++u) {
+        for (int u = 0; u < HEADS; ++u) {
             x[u][0] = x[u][1] = make_uint2(0u, 0u);
             if (first + u * kSegments < p.heads && holds) {
                 x[u][0] = *reinterpret_cast<const uint2*>(from[u] + 2 * at0);
@@ -145,7 +147,7 @@ __global__ void __launch_bounds__(kThreads, 2) append_kernel(const AppendParams 
         f[3] = b[1];
     };
 
-    uint2 x[kHeadsPerLane][2];
+    uint2 x[HEADS][2];
     load(x);
     if (tid / 32 < tokens) {
         const int token = token0 + tid / 32;
@@ -174,7 +176,7 @@ __global__ void __launch_bounds__(kThreads, 2) append_kernel(const AppendParams 
 #pragma unroll 1
     for (int i = 0; i < tokens; ++i) {
         const Place place = s_place[i];
-        uint2 ahead[kHeadsPerLane][2];
+        uint2 ahead[HEADS][2];
         float4 cs_ahead = {}, sn_ahead = {};
         if (i + 1 < tokens) {
             load(ahead);
@@ -185,7 +187,7 @@ __global__ void __launch_bounds__(kThreads, 2) append_kernel(const AppendParams 
             const float2 c2[2] = {make_float2(cs.x, cs.y), make_float2(cs.z, cs.w)};
             const float2 s2[2] = {make_float2(sn.x, sn.y), make_float2(sn.z, sn.w)};
 #pragma unroll
-            for (int u = 0; u < kHeadsPerLane; ++u) {
+            for (int u = 0; u < HEADS; ++u) {
                 const int h = first + u * kSegments;
                 const bool is_value = h >= v_begin;
                 uint2 y[2] = {x[u][0], x[u][1]};  // values bit for bit, NaN payloads included
@@ -252,7 +254,7 @@ __global__ void __launch_bounds__(kThreads, 2) append_kernel(const AppendParams 
             }
         }
 #pragma unroll
-        for (int u = 0; u < kHeadsPerLane; ++u) {
+        for (int u = 0; u < HEADS; ++u) {
             x[u][0] = ahead[u][0];
             x[u][1] = ahead[u][1];
             if (first + u * kSegments < k_begin) to[u] += 2 * p.q_out_token;
@@ -262,15 +264,21 @@ __global__ void __launch_bounds__(kThreads, 2) append_kernel(const AppendParams 
     }
 }
 
-template <typename T>
-cudaError_t launch_append(const AppendParams& p, unsigned blocks, bool narrow, cudaStream_t stream) {
+template <typename T, int LANES>
+cudaError_t launch_append(const AppendParams& p, unsigned blocks, int heads_per_lane, cudaStream_t stream) {
     KernelTimer timer("kv_append", stream);
-    if (narrow) {
-        append_kernel<T, 8><<<blocks, kThreads, 0, stream>>>(p);
-    } else {
-        append_kernel<T, 16><<<blocks, kThreads, 0, stream>>>(p);
+    switch (heads_per_lane) {
+        case 1: append_kernel<T, LANES, 1><<<blocks, kThreads, 0, stream>>>(p); break;
+        case 2: append_kernel<T, LANES, 2><<<blocks, kThreads, 0, stream>>>(p); break;
+        case 3: append_kernel<T, LANES, 3><<<blocks, kThreads, 0, stream>>>(p); break;
+        default: append_kernel<T, LANES, 4><<<blocks, kThreads, 0, stream>>>(p); break;
     }
     return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t launch_append_any(const AppendParams& p, unsigned blocks, int heads_per_lane, cudaStream_t stream) {
+    return p.view.head_dim <= 64 ? launch_append<T, 8>(p, blocks, heads_per_lane, stream) : launch_append<T, 16>(p, blocks, heads_per_lane, stream);
 }
 
 }  // namespace
@@ -318,10 +326,10 @@ extern "C" int zcgvs_kv_append(const zcgvs_paged_cache* cache, const zcgvs_step_
     } else {
         rotary_dim = 16;  // not used
     }
-    const bool narrow = cache->head_dim <= 64;
-    const int per_block = kThreads / (narrow ? 8 : 16) * kHeadsPerLane;
+    const int segments = kThreads / (cache->head_dim <= 64 ? 8 : 16);
     const long long heads = static_cast<long long>(q_heads) + (k != nullptr ? 2LL * cache->kv_heads : 0);
-    const long long chunks = (heads + per_block - 1) / per_block;
+    const int heads_per_lane = static_cast<int>(std::min<long long>((heads + segments - 1) / segments, kMaxHeads));
+    const long long chunks = (heads + segments * heads_per_lane - 1) / (segments * heads_per_lane);
     if (heads > INT_MAX / 2 || chunks * batch->tokens > INT_MAX) return invalid(what, "too many tokens and heads for one call");
     p.q = static_cast<const uint8_t*>(q);
     p.k = static_cast<const uint8_t*>(k);
@@ -351,8 +359,8 @@ extern "C" int zcgvs_kv_append(const zcgvs_paged_cache* cache, const zcgvs_step_
     p.tokens_per_block = static_cast<int>(std::min<long long>(std::max<long long>(chunks * batch->tokens / fill, 1), kMaxTokens));
     const unsigned blocks = static_cast<unsigned>(chunks * ((batch->tokens + p.tokens_per_block - 1) / p.tokens_per_block));
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const cudaError_t e = cache->dtype == ZCGVS_DTYPE_F16 ? launch_append<__half>(p, blocks, narrow, s)
-                                                          : launch_append<__nv_bfloat16>(p, blocks, narrow, s);
+    const cudaError_t e = cache->dtype == ZCGVS_DTYPE_F16 ? launch_append_any<__half>(p, blocks, heads_per_lane, s)
+                                                          : launch_append_any<__nv_bfloat16>(p, blocks, heads_per_lane, s);
     if (e != cudaSuccess) return fail_cuda(e, what);
     return ok();
 }
