@@ -158,10 +158,12 @@ def _ptr(t):
 
 
 def _stream(stream):
+    if stream is not None:
+        return ctypes.c_void_p(stream.cuda_stream)
     import torch
 
-    s = torch.cuda.current_stream() if stream is None else stream
-    return ctypes.c_void_p(s.cuda_stream)
+    # The current stream's handle alone: building torch's Stream object for it takes 3.5 us.
+    return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
 
 
 class Workspace:
@@ -621,21 +623,19 @@ def _value_dtype(t, name: str, f32: bool = False) -> int:
     return code
 
 
-def _on_device(device, **tensors):
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            _refuse(f"{name} is on {t.device}, not on {device}")
-
-
-def _typed(t, name: str, dtype, shape=None):
+def _side(t, name: str, device, dtype, shape=None):
+    """The address of an optional contiguous operand of a given type and shape, or None."""
     if t is None:
-        return
+        return None
     if t.dtype != dtype:
         _refuse(f"{name} must be {dtype}, not {t.dtype}")
     if not t.is_contiguous():
         _refuse(f"{name} must be contiguous")
-    if shape is not None and tuple(t.shape) != shape:
+    if shape is not None and t.shape != shape:
         _refuse(f"{name} must have shape {shape}, not {tuple(t.shape)}")
+    if t.device != device:
+        _refuse(f"{name} is on {t.device}, not on {device}")
+    return t.data_ptr()
 
 
 class PagedKvCache:
@@ -647,8 +647,10 @@ class PagedKvCache:
             _refuse("PagedKvCache: keys and values must be 4-D views of the same shape, strides and type")
         if keys.shape[3] > 1 and keys.stride(3) != 1:
             _refuse("PagedKvCache: the elements of a head must be contiguous")
-        _on_device(keys.device, values=values)
+        if values.device != keys.device:
+            _refuse(f"values are on {values.device}, not on {keys.device}")
         self.keys, self.values = keys, values
+        self.device, self.dtype = keys.device, keys.dtype
         self.pages, self.page_size, self.kv_heads, self.head_dim = keys.shape
         self.struct = _PagedCacheStruct(keys.data_ptr(), values.data_ptr(), self.pages, keys.stride(0), keys.stride(1),
                                         keys.stride(2), self.page_size, self.kv_heads, self.head_dim,
@@ -667,12 +669,14 @@ class StepBatch:
         import torch
 
         n = kv_lengths.numel()
-        _typed(query_starts, "query_starts", torch.int32, (n + 1,))
-        _typed(kv_lengths, "kv_lengths", torch.int32, (n,))
+        self.device = kv_lengths.device
+        _side(query_starts, "query_starts", self.device, torch.int32, (n + 1,))
+        _side(kv_lengths, "kv_lengths", self.device, torch.int32, (n,))
         if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != n or \
                 (page_table.shape[1] > 1 and page_table.stride(1) != 1):
             _refuse("page_table must be int32 [sequences, pages] with contiguous rows")
-        _on_device(kv_lengths.device, query_starts=query_starts, page_table=page_table)
+        if page_table.device != self.device:
+            _refuse(f"page_table is on {page_table.device}, not on {self.device}")
         self.query_starts, self.kv_lengths, self.page_table = query_starts, kv_lengths, page_table
         self.tokens, self.sequences = int(tokens), n
         columns = page_table.shape[1]
@@ -687,16 +691,24 @@ def _rows(t, name: str, cache: PagedKvCache, batch: StepBatch, heads: int | None
     """(pointer, token stride, head stride) of a [tokens, heads, head_dim] operand."""
     if t is None:
         return None, 0, 0
-    if t.dim() != 3 or t.shape[0] != batch.tokens or t.shape[2] != cache.head_dim or (heads is not None and t.shape[1] != heads):
+    shape = t.shape
+    if len(shape) != 3 or shape[0] != batch.tokens or shape[2] != cache.head_dim or (heads is not None and shape[1] != heads):
         _refuse(f"{name} must be [{batch.tokens}, {heads if heads is not None else 'heads'}, {cache.head_dim}], "
-                f"not {tuple(t.shape)}")
-    if t.dtype != cache.keys.dtype:
-        _refuse(f"{name} must have the cache's type {cache.keys.dtype}, not {t.dtype}")
-    if cache.head_dim > 1 and t.stride(2) != 1:
+                f"not {tuple(shape)}")
+    if t.dtype != cache.dtype:
+        _refuse(f"{name} must have the cache's type {cache.dtype}, not {t.dtype}")
+    if t.device != cache.device:
+        _refuse(f"{name} is on {t.device}, not on {cache.device}")
+    token_stride, head_stride, step = t.stride()
+    if step != 1 and cache.head_dim > 1:
         _refuse(f"{name}: the elements of a head must be contiguous")
-    _on_device(cache.keys.device, **{name: t})
     # The stride of an axis of one entry means nothing; 0 passes the library's checks.
-    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else 0, t.stride(1) if t.shape[1] > 1 else 0
+    return t.data_ptr(), token_stride if shape[0] > 1 else 0, head_stride if shape[1] > 1 else 0
+
+
+def _same_device(cache: PagedKvCache, batch: StepBatch):
+    if batch.device != cache.device:
+        _refuse(f"the step is on {batch.device}, not on {cache.device}")
 
 
 def rotary_table(rows: int, rotary_dim: int, base: float = 10000.0, device=None):
@@ -716,26 +728,30 @@ def kv_append(cache: PagedKvCache, batch: StepBatch, q, k, v, *, rotary=None, in
     values in the paged cache. Returns the queries (`out`, which may be q), or None without q."""
     import torch
 
-    device = cache.keys.device
-    _on_device(device, kv_lengths=batch.kv_lengths, rotary=rotary, q_norm=q_norm, k_norm=k_norm, positions=positions)
-    _typed(rotary, "rotary", torch.float32)
-    _typed(q_norm, "q_norm", cache.keys.dtype, (cache.head_dim,))
-    _typed(k_norm, "k_norm", cache.keys.dtype, (cache.head_dim,))
-    _typed(positions, "positions", torch.int32, (batch.tokens,))
+    _same_device(cache, batch)
+    device = cache.device
     if rotary is not None and rotary.dim() != 2:
         _refuse("rotary must be [rows, rotary_dim]")
+    rotary_ptr = _side(rotary, "rotary", device, torch.float32)
+    q_norm_ptr = _side(q_norm, "q_norm", device, cache.dtype, (cache.head_dim,))
+    k_norm_ptr = _side(k_norm, "k_norm", device, cache.dtype, (cache.head_dim,))
+    positions_ptr = _side(positions, "positions", device, torch.int32, (batch.tokens,))
     q_args = _rows(q, "q", cache, batch)
     k_args = _rows(k, "k", cache, batch, cache.kv_heads)
     v_args = _rows(v, "v", cache, batch, cache.kv_heads)
-    heads = 0 if q is None else q.shape[1]
-    if q is not None and out is None:
-        out = torch.empty((batch.tokens, heads, cache.head_dim), dtype=q.dtype, device=device)
-    o_args = _rows(out if q is not None else None, "out", cache, batch, heads)
+    heads = 0
+    if q is None:
+        out = None
+    else:
+        heads = q.shape[1]
+        if out is None:
+            out = torch.empty_like(q)
+    o_args = _rows(out, "out", cache, batch, heads)
     rows, width = (0, 0) if rotary is None else rotary.shape
-    check(lib().zcgvs_kv_append(cache.ref, batch.ref, *q_args, heads, *k_args, *v_args, _ptr(q_norm), _ptr(k_norm), eps,
-                                _ptr(rotary), rows, width, 1 if interleaved else 0, _ptr(positions), *o_args,
+    check(lib().zcgvs_kv_append(cache.ref, batch.ref, *q_args, heads, *k_args, *v_args, q_norm_ptr, k_norm_ptr, eps,
+                                rotary_ptr, rows, width, 1 if interleaved else 0, positions_ptr, *o_args,
                                 _stream(stream)))
-    return out if q is not None else None
+    return out
 
 
 _attention_bytes: dict[tuple[int, int], int] = {}
@@ -751,14 +767,14 @@ def paged_attention(cache: PagedKvCache, batch: StepBatch, q, *, scale: float, c
     output, with return_lse (output, fp32 [tokens, q_heads] log-sum-exp)."""
     import torch
 
-    device = cache.keys.device
-    _on_device(device, kv_lengths=batch.kv_lengths)
+    _same_device(cache, batch)
+    device = cache.device
     if q is None:
         _refuse("q must be given")
     q_args = _rows(q, "q", cache, batch)
     heads = q.shape[1]
     if out is None:
-        out = torch.empty((batch.tokens, heads, cache.head_dim), dtype=q.dtype, device=device)
+        out = torch.empty_like(q)
     o_args = _rows(out, "out", cache, batch, heads)
     lse = torch.empty((batch.tokens, heads), dtype=torch.float32, device=device) if return_lse else None
     ws, owned = _own_workspace(workspace, device)
@@ -768,7 +784,8 @@ def paged_attention(cache: PagedKvCache, batch: StepBatch, q, *, scale: float, c
         nbytes = _attention_bytes[key] = paged_attention_workspace_bytes(cache.head_dim)
     buf = ws.get(nbytes, stream)
     check(lib().zcgvs_paged_attention(cache.ref, batch.ref, *q_args, heads, scale, 1 if causal else 0, window, *o_args,
-                                      _ptr(lse), _ptr(buf), buf.numel(), _stream(stream)))
+                                      None if lse is None else lse.data_ptr(), buf.data_ptr(), buf.numel(),
+                                      _stream(stream)))
     if owned:
         ws.raise_on_status(stream)
     return (out, lse) if return_lse else out
@@ -784,14 +801,16 @@ def sample(logits, uniforms, *, temperature=None, top_k=None, top_p=None, min_p=
         _refuse("logits must be [rows, vocab] with contiguous rows")
     rows, vocab = logits.shape
     dtype = _value_dtype(logits, "logits", f32=True)
-    for name, t in (("uniforms", uniforms), ("temperature", temperature), ("top_p", top_p), ("min_p", min_p)):
-        _typed(t, name, torch.float32, (rows,))
-    _typed(top_k, "top_k", torch.int32, (rows,))
-    _on_device(logits.device, uniforms=uniforms, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+    if uniforms is None:
+        _refuse("uniforms must be given")
+    device, shape = logits.device, (rows,)
+    u, t, p, m = (_side(x, name, device, torch.float32, shape) for x, name in
+                  ((uniforms, "uniforms"), (temperature, "temperature"), (top_p, "top_p"), (min_p, "min_p")))
+    k = _side(top_k, "top_k", device, torch.int32, shape)
     if out is None:
-        out = (torch.empty((rows,), dtype=torch.int32, device=logits.device),
-               torch.empty((rows,), dtype=torch.float32, device=logits.device))
-    check(lib().zcgvs_sample(_ptr(logits), dtype, logits.stride(0) if rows > 1 else vocab, rows, vocab, _ptr(temperature),
-                             _ptr(top_k), _ptr(top_p), _ptr(min_p), _ptr(uniforms), _ptr(out[0]), _ptr(out[1]),
-                             _stream(stream)))
+        out = (torch.empty(shape, dtype=torch.int32, device=device), torch.empty(shape, dtype=torch.float32, device=device))
+    tokens = _side(out[0], "out[0]", device, torch.int32, shape)
+    logprobs = _side(out[1], "out[1]", device, torch.float32, shape)
+    check(lib().zcgvs_sample(logits.data_ptr(), dtype, logits.stride(0) if rows > 1 else vocab, rows, vocab, t, k, p, m, u,
+                             tokens, logprobs, _stream(stream)))
     return out
