@@ -18,6 +18,9 @@
 //     rescaled, in tensor memory) only when the maximum rose by more than 8 in log2 units, so
 //     weights stay below 2^8 and rescaling is rare; the result is the same, since sum and O share
 //     the reference point.
+//   * Warp 10 walks this CTA's part of the line and hands every stay at a unit to the other roles
+//     through a ring in shared memory. (Walked by each role for itself, the walk's registers spilled
+//     in all of them: a wait of the issuing warp then took 150 to 400 cycles.)
 //   * Warps 12-15 write a finished unit's O while the softmax warps are at the next unit (done by
 //     the softmax warps, a unit cost about 4 us more).
 // Tensor memory: S_0, S_1 (P over them) and O_0, O_1, 128 columns each.
@@ -41,10 +44,12 @@ namespace paged {
 constexpr int kChunkRows = 256;
 constexpr int kChunkKeys = 128;
 constexpr int kChunkExtra = 3;  // a unit's first loads and its end, in tiles
-constexpr int kChunkThreads = 512;  // warps 10 and 11 only complete their warpgroup
+constexpr int kChunkThreads = 512;  // warp 11 only completes its warpgroup
 constexpr int kProducerWarp = 8;
 constexpr int kIssueWarp = 9;
+constexpr int kPlanWarp = 10;
 constexpr int kOutputWarp = 12;  // to 15
+constexpr int kWorkSlots = 4;
 // Registers: the launch gives 128 to each of 512 threads (65,536); the softmax warpgroups hold a
 // row's 128 scores and take 192, the other two give up the difference: 256 * 192 + 256 * 64 = 65,536.
 constexpr int kSoftmaxRegisters = 192;
@@ -164,7 +169,22 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 __device__ __forceinline__ void give_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegisters)); }
 __device__ __forceinline__ void take_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters)); }
 
+// A CTA's stay at one unit, as the roles need it.
+struct Work {
+    int sequence;     // -1: no more work
+    int head;
+    int token0, row0; // the sequence's first token; the unit's first row, of the sequence
+    int rows;         // rows of the unit that exist, at most 256
+    int lo, hi;       // the unit's keys
+    int pos0, tiles;  // first position of the first key tile, and how many
+    int before;       // position of the sequence's first new token
+    int cap;          // keys that exist
+    int slot;         // of the partial result; -1: the whole unit is here
+};
+
 struct ChunkShared {
+    Work work[kWorkSlots];
+    u64 work_full[kWorkSlots], work_empty[kWorkSlots];
     u64 kv_full[8], kv_empty[8];
     u64 raw;  // a value tile that the producer still has to clear rows of
     u64 q_full[2], q_empty[2], s_full[2], o_full[2];
@@ -224,6 +244,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             mbar_init(&sh.kv_full[s], 1);
             mbar_init(&sh.kv_empty[s], 1);
         }
+        for (int i = 0; i < kWorkSlots; ++i) {
+            mbar_init(&sh.work_full[i], 1);
+            mbar_init(&sh.work_empty[i], 14);  // producer, products, softmax and output warps
+        }
         mbar_init(&sh.raw, 1);
         for (int h = 0; h < 2; ++h) {
             mbar_init(&sh.q_full[h], q_by_tma ? 1 : 128);
@@ -248,7 +272,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     fence_after();
     const uint32_t tmem = sh.tmem;
     volatile int* abort_flag = &sh.abort;
-    Segment g = plan_shared.segment;
 
     // Waits for a phase, or gives up for the whole CTA.
     auto wait = [&](u64* bar, uint32_t parity, uint32_t flag) {
@@ -260,6 +283,13 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         return true;
     };
 
+    // The i-th stay of this CTA, once it is there; and a warp's word that it is done with it.
+    auto take = [&](uint32_t i) { return __all_sync(0xffffffffu, wait(&sh.work_full[i % kWorkSlots], (i / kWorkSlots) & 1u, kStatusHandOff)) != 0; };
+    auto give = [&](uint32_t i) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cta(&sh.work_empty[i % kWorkSlots]);
+    };
+
     if (warp >= kOutputWarp) {
         // ---------------- output ----------------
         give_registers();
@@ -269,17 +299,16 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         uint32_t step[2] = {0u, 0u};      // tiles of each half, over all segments
         uint32_t segments[2] = {0u, 0u};  // those each half works in
         bool ok = true;
-        for (bool more = true; more && ok;) {
-            const int rows = g.seq.n * p.group - g.rt * kChunkRows;  // live rows of the unit, if below 256
-            const bool whole_unit = g.begin == 0 && g.end == g.range.count;
-            const int slot = plan.slot(blockIdx.x, g.unit_start);
-            if (tid == kOutputWarp * 32 && !whole_unit && g.begin == 0) {
-                const long long last = (g.unit_start + g.range.count - 1) / plan.quota;
-                joins[blockIdx.x] = {g.seq.begin, g.seq.n, g.rt, g.head, slot, static_cast<int>(last - blockIdx.x) + 1};
-            }
+        for (uint32_t stay = 0; ok; ++stay) {
+            ok = take(stay);
+            if (!ok) break;
+            const Work& w = sh.work[stay % kWorkSlots];
+            if (w.sequence < 0) break;
+            const int rows = w.rows;
+            const bool whole_unit = w.slot < 0;
             for (int h = 0; h < 2 && ok; ++h) {
                 if (h * 128 >= rows) break;
-                step[h] += g.end - g.begin;
+                step[h] += w.tiles;
                 // Through shared memory, so that a store covers 64 bytes of each of 8 rows (one row
                 // per thread would touch 32 lines with every store). Lane i writes 16 bytes of rows
                 // i / 4 + {0, 8, 16, 24} of the warp's.
@@ -288,9 +317,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int in_unit = first + i * 8 + (lane >> 2);
-                    const int of = g.rt * kChunkRows + in_unit;
+                    const int of = w.row0 + in_unit;
                     const int j = p.by_group.quotient(of);
-                    to[i] = in_unit < rows ? (g.seq.begin + j) * p.out_token + (g.head * p.group + of - j * p.group) * p.out_head : -1;
+                    to[i] = in_unit < rows ? (w.token0 + j) * p.out_token + (w.head * p.group + of - j * p.group) * p.out_head : -1;
                 }
                 ok = wait(&sh.stats_full[h], segments[h] & 1u, kStatusHandOff) && wait(&sh.o_full[h], (step[h] - 1u) & 1u, kStatusHandOff);
                 ++segments[h];
@@ -303,9 +332,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                 if (whole_unit) {
                     const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
                     if (h * 128 + r < rows && p.lse != nullptr) {
-                        const int row = g.rt * kChunkRows + h * 128 + r;
+                        const int row = w.row0 + h * 128 + r;
                         const int j = p.by_group.quotient(row);
-                        p.lse[static_cast<long long>(g.seq.begin + j) * p.q_heads + g.head * p.group + row - j * p.group] =
+                        p.lse[static_cast<long long>(w.token0 + j) * p.q_heads + w.head * p.group + row - j * p.group] =
                             sum > 0.0f ? (stats.x + log2f(sum)) * 0.69314718056f : (sum == 0.0f ? -INFINITY : sum);
                     }
 #pragma unroll 1
@@ -344,19 +373,16 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                         tmem_load_wait();
 #pragma unroll
                         for (int i = 0; i < 32; i += 4) {
-                            *reinterpret_cast<float4*>(p.part_o + part_at<DP>(slot, (c + i) / 4, h * 128 + r)) =
+                            *reinterpret_cast<float4*>(p.part_o + part_at<DP>(w.slot, (c + i) / 4, h * 128 + r)) =
                                 make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
                         }
                     }
-                    *reinterpret_cast<float2*>(p.part_ml + (static_cast<long long>(slot) * kChunkRows + h * 128 + r) * 2) = stats;
+                    *reinterpret_cast<float2*>(p.part_ml + (static_cast<long long>(w.slot) * kChunkRows + h * 128 + r) * 2) = stats;
                 }
                 fence_before();
                 mbar_arrive_cta(&sh.o_free[h]);
             }
-            if (!ok) break;
-            Segment following;
-            more = plan.next(g, following);
-            g = following;
+            give(stay);
         }
     } else if (warp >= kProducerWarp) {
     give_registers();
@@ -374,26 +400,28 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             bool mine;
             int page, slot;
         };
-        auto find = [&](const Segment& of, int t) {
-            const int pos = (of.range.first + t) * kChunkKeys + lane * box;
-            Box b{lane < boxes && pos < of.range.hi && pos + box > of.range.lo, -1, 0};
+        auto find = [&](const Work& of, int t) {
+            const int pos = of.pos0 + t * kChunkKeys + lane * box;
+            Box b{lane < boxes && pos < of.hi && pos + box > of.lo, -1, 0};
             if (b.mine) {
                 const int column = page_column(view, pos);
-                b.page = __ldg(view.table + of.s * view.table_stride + column);
+                b.page = __ldg(view.table + of.sequence * view.table_stride + column);
                 b.slot = pos - column * view.page_size;
             }
             return b;
         };
-        Box ahead = find(g, g.begin);
-        for (bool more = true; more && ok;) {
-            Segment following;
-            more = plan.next(g, following);
+        ok = take(0);
+        Box ahead{};
+        if (ok) ahead = find(sh.work[0], 0);
+        for (uint32_t stay = 0; ok; ++stay) {
+            const Work& w = sh.work[stay % kWorkSlots];
+            if (w.sequence < 0) break;
+            const int head = w.head, tiles = w.tiles;
             if (q_by_tma) {
                 // 128 rows are 128 / group whole tokens of one head group. Tokens past the sequence's
                 // (or, as zeros, past all) belong to rows whose results are dropped.
                 for (int h = 0; h < 2 && ok; ++h) {
-                    const int row = g.rt * kChunkRows + h * 128;
-                    if (row >= g.seq.n * p.group) break;
+                    if (h * 128 >= w.rows) break;
                     if (queries[h] > 0) ok = __all_sync(0xffffffffu, wait(&sh.q_empty[h], (queries[h] - 1u) & 1u, kStatusHandOff));
                     if (!ok) break;
                     ++queries[h];
@@ -401,24 +429,26 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                         mbar_arrive_expect_tx(&sh.q_full[h], kQBytes);
 #pragma unroll
                         for (int c = 0; c < kHalves; ++c) {
-                            load_queries_box(q_smem + h * kQBytes + c * kColumnBytes, &map_q, c * 64, g.head * p.group,
-                                             g.seq.begin + p.by_group.quotient(row), &sh.q_full[h]);
+                            load_queries_box(q_smem + h * kQBytes + c * kColumnBytes, &map_q, c * 64, head * p.group,
+                                             w.token0 + p.by_group.quotient(w.row0 + h * 128), &sh.q_full[h]);
                         }
                     }
                     __syncwarp();
                 }
                 if (!ok) break;
             }
-            for (int t = g.begin; t < g.end && ok; ++t) {
-                const int pos0 = (g.range.first + t) * kChunkKeys;
-                const bool partial = pos0 < g.range.lo || pos0 + kChunkKeys > g.range.hi;
+            for (int t = 0; t < tiles && ok; ++t) {
+                const int pos0 = w.pos0 + t * kChunkKeys;
+                const bool partial = pos0 < w.lo || pos0 + kChunkKeys > w.hi;
                 const Box now = ahead;
                 const bool mine = now.mine;
                 const int page = now.page, slot = now.slot;
-                if (t + 1 < g.end) {
-                    ahead = find(g, t + 1);
-                } else if (more) {
-                    ahead = find(following, following.begin);
+                if (t + 1 < tiles) {
+                    ahead = find(w, t + 1);
+                } else {
+                    ok = take(stay + 1);
+                    const Work& following = sh.work[(stay + 1) % kWorkSlots];
+                    if (ok && following.sequence >= 0) ahead = find(following, 0);
                 }
                 const int count = __popc(__ballot_sync(0xffffffffu, mine));
                 for (int which = 0; which < 2 && ok; ++which) {  // the keys, then the values
@@ -434,7 +464,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                     if (mine) {
 #pragma unroll
                         for (int c = 0; c < kHalves; ++c) {
-                            load_box(dst + c * kColumnBytes + lane * box_bytes, which == 0 ? &map_k : &map_v, c * 64, slot, g.head, page, bar);
+                            load_box(dst + c * kColumnBytes + lane * box_bytes, which == 0 ? &map_k : &map_v, c * 64, slot, head, page, bar);
                         }
                     }
                     ++used;
@@ -447,7 +477,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                             *abort_flag = 1;
                             break;
                         }
-                        const int a = max(g.range.lo - pos0, 0), b = min(max(g.range.hi - pos0, 0), kChunkKeys);
+                        const int a = max(w.lo - pos0, 0), b = min(max(w.hi - pos0, 0), kChunkKeys);
                         for (int i = lane; i < kChunkKeys * 8 * kHalves; i += 32) {
                             const int row = (i >> 3) & (kChunkKeys - 1);
                             if (row < a || row >= b) {
@@ -461,7 +491,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                     }
                 }
             }
-            g = following;
+            give(stay);
         }
         if (*abort_flag) {
             // Copies in flight land before the CTA retires. Slots of cleared tiles have completed already.
@@ -516,9 +546,14 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             }
             __syncwarp();
         };
-        for (bool more = true; more && ok;) {
-            const int halves = __shfl_sync(0xffffffffu, g.seq.n * p.group - g.rt * kChunkRows > 128 ? 2 : 1, 0);
-            const int tiles = __shfl_sync(0xffffffffu, g.end - g.begin, 0);
+        for (uint32_t stay = 0; ok; ++stay) {
+            ok = take(stay);
+            if (!ok) break;
+            const Work& w = sh.work[stay % kWorkSlots];
+            const int halves = __shfl_sync(0xffffffffu, w.rows > 128 ? 2 : 1, 0);
+            const int tiles = __shfl_sync(0xffffffffu, w.sequence < 0 ? 0 : w.tiles, 0);
+            if (tiles == 0) break;
+            give(stay);
             // Slots of this segment: keys of tile t at used + 2 t, values at used + 2 t + 1.
             ok = slot_full(used);
 #pragma unroll
@@ -548,14 +583,48 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                 }
             }
             used += 2 * tiles;
-            Segment following;
-            more = plan.next(g, following);
-            g = following;
         }
         // No product is in flight when tensor memory is freed.
         if (elected()) commit_to(&sh.drain);
         __syncwarp();
         mbar_wait_bounded(&sh.drain, 0u, p.status, kStatusDrainTimeout);
+    } else if (warp == kPlanWarp) {
+        // ---------------- plan ----------------
+        Segment g = plan_shared.segment;
+        bool more = true;
+        for (uint32_t stay = 0;; ++stay) {
+            if (stay >= kWorkSlots && !__all_sync(0xffffffffu, wait(&sh.work_empty[stay % kWorkSlots], (stay / kWorkSlots - 1u) & 1u, kStatusHandOff))) break;
+            if (lane == 0) {
+                Work w{};
+                w.sequence = -1;
+                if (more) {
+                    const bool whole_unit = g.begin == 0 && g.end == g.range.count;
+                    w.sequence = g.s;
+                    w.head = g.head;
+                    w.token0 = g.seq.begin;
+                    w.row0 = g.rt * kChunkRows;
+                    w.rows = min(g.seq.n * p.group - w.row0, kChunkRows);
+                    w.lo = g.range.lo;
+                    w.hi = g.range.hi;
+                    w.pos0 = (g.range.first + g.begin) * kChunkKeys;
+                    w.tiles = g.end - g.begin;
+                    w.before = g.seq.length - g.seq.n;
+                    w.cap = static_cast<int>(min(static_cast<long long>(g.seq.length), static_cast<long long>(view.table_cols) * view.page_size));
+                    w.slot = whole_unit ? -1 : plan.slot(blockIdx.x, g.unit_start);
+                    if (!whole_unit && g.begin == 0) {
+                        const long long last = (g.unit_start + g.range.count - 1) / plan.quota;
+                        joins[blockIdx.x] = {g.seq.begin, g.seq.n, g.rt, g.head, w.slot, static_cast<int>(last - blockIdx.x) + 1};
+                    }
+                }
+                sh.work[stay % kWorkSlots] = w;
+                mbar_arrive_cta(&sh.work_full[stay % kWorkSlots]);
+            }
+            __syncwarp();
+            if (!more) break;
+            Segment following;
+            more = plan.next(g, following);
+            g = following;
+        }
     }
     } else {
         // ---------------- softmax ----------------
@@ -572,9 +641,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         // Brings the rows of this half of a unit to shared memory where TMA boxes do not fit them (a
         // group that is no power of two), 16 bytes per thread and row; all loads of a batch are in
         // flight together.
-        auto load_queries = [&](const Segment& of) {
+        auto load_queries = [&](const Work& of) {
             constexpr int kPieces = DP / 8, kStep = 128 / kPieces, kBatch = 8;
-            const int rows = of.seq.n * p.group - of.rt * kChunkRows - h * 128;  // live ones
+            const int rows = of.rows - h * 128;  // that exist
             const int piece = r % kPieces, row0 = r / kPieces;
             const bool inside = piece * 8 < view.head_dim;
 #pragma unroll
@@ -583,9 +652,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
 #pragma unroll
                 for (int i = 0; i < kBatch; ++i) {
                     const int rr = row0 + (b + i) * kStep;
-                    const int global = of.rt * kChunkRows + h * 128 + rr;
+                    const int global = of.row0 + h * 128 + rr;
                     const int j = p.by_group.quotient(global);
-                    const long long token = of.seq.begin + j;
+                    const long long token = of.token0 + j;
                     const int head = of.head * p.group + global - j * p.group;
                     v[i] = make_uint4(0u, 0u, 0u, 0u);
                     if (rr < rows && inside) v[i] = __ldg(reinterpret_cast<const uint4*>(p.q + 2 * (token * p.q_token + head * p.q_head + piece * 8)));
@@ -602,26 +671,27 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             fence_proxy_async_shared();
             mbar_arrive_cta(&sh.q_full[h]);
         };
-        auto half_works = [&](const Segment& of) { return h == 0 || of.seq.n * p.group - of.rt * kChunkRows > 128; };
-
-        if (!q_by_tma && half_works(g)) load_queries(g);
-        for (bool more = true; more;) {
-            const int rows = g.seq.n * p.group - g.rt * kChunkRows;  // live rows of the unit, if below 256
-            const bool works = half_works(g);
-            const int row = g.rt * kChunkRows + h * 128 + r;  // of the sequence
-            const bool live = h * 128 + r < rows;
-            bool ok = true;
+        bool ok = take(0);
+        if (ok && !q_by_tma && h * 128 < sh.work[0].rows) load_queries(sh.work[0]);
+        for (uint32_t stay = 0; ok; ++stay) {
+            ok = take(stay);
+            if (!ok) break;
+            const Work& w = sh.work[stay % kWorkSlots];
+            if (w.sequence < 0) break;
+            const bool works = h * 128 < w.rows;
+            const bool live = h * 128 + r < w.rows;
             float top = -INFINITY, sum = 0.0f;  // reference point (raw score units), sum of weights
             if (works) {
-                const int cap = static_cast<int>(min(static_cast<long long>(g.seq.length), static_cast<long long>(view.table_cols) * view.page_size));
-                int lo, hi;
-                row_range(p, g.seq, row, cap, lo, hi);
-                if (!live) lo = hi = 0;
+                const int pos = w.before + p.by_group.quotient(w.row0 + h * 128 + r);  // of this row's token
+                int hi = pos < 0 || !live ? 0 : p.causal ? min(w.cap, pos + 1) : w.cap;
+                int lo = live && p.window > 0 && pos >= p.window ? pos - p.window + 1 : 0;
+                int pos0 = w.pos0;
+                const int tiles = w.tiles;
                 // A tile inside the range of every live row of the warp needs no mask; padding rows'
                 // queries are zeros and their results are dropped.
                 const int all_lo = __reduce_max_sync(0xffffffffu, live ? lo : 0), all_hi = __reduce_min_sync(0xffffffffu, live ? hi : INT_MAX);
 
-                for (int t = g.begin; t < g.end && ok; ++t, ++step) {
+                for (int t = 0; t < tiles && ok; ++t, ++step, pos0 += kChunkKeys) {
                     ok = __all_sync(0xffffffffu, wait(&sh.s_full[h], step & 1u, kStatusHandOff));
                     if (!ok) break;
                     fence_after();
@@ -629,7 +699,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
 #pragma unroll
                     for (int c = 0; c < 4; ++c) tmem_load32(s_addr + c * 32, s + c * 32);
                     tmem_load_wait();
-                    const int pos0 = (g.range.first + t) * kChunkKeys;
                     const bool masked = pos0 < all_lo || pos0 + kChunkKeys > all_hi;
                     if (masked) {
                         const auto below = [](int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; };
@@ -658,8 +727,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                         top = best;
                     }
                     if (__any_sync(0xffffffffu, shrink != 1.0f)) {
-                        // O holds the tiles before this one; its last product must be done. (t >
-                        // g.begin here: top was -inf at the first.)
+                        // O holds the tiles before this one; its last product must be done. (t > 0
+                        // here: top was -inf at the first.)
                         ok = __all_sync(0xffffffffu, wait(&sh.o_full[h], (step - 1u) & 1u, kStatusHandOff));
                         if (!ok) break;
                         fence_after();
@@ -696,13 +765,14 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                     sum += part[0].x + part[0].y;
                 }
             }
-            Segment following;
-            more = plan.next(g, following);
-            if (ok && more && !q_by_tma) {
+            give(stay);
+            if (ok && !q_by_tma) {
                 // The products that read this half's queries are done (its last scores were waited
                 // for), so the next unit's scores can start while this one's output is written. A
                 // half that did not work in this unit was waited for in an earlier one.
-                if (half_works(following)) load_queries(following);
+                ok = take(stay + 1);
+                const Work& following = sh.work[(stay + 1) % kWorkSlots];
+                if (ok && following.sequence >= 0 && h * 128 < following.rows) load_queries(following);
             }
             if (works && ok) {
                 if (segments > 0) ok = __all_sync(0xffffffffu, wait(&sh.o_free[h], (segments - 1u) & 1u, kStatusHandOff));
@@ -710,12 +780,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                 sh.stats[h][r] = make_float2(top == -INFINITY ? top : top * scale, sum);
                 mbar_arrive_cta(&sh.stats_full[h]);
             }
-            if (!ok) {
-                *abort_flag = 1;
-                break;
-            }
-            g = following;
         }
+        if (!ok) *abort_flag = 1;
     }
 
     fence_before();
