@@ -70,13 +70,13 @@ struct Shared {
     float top;                 // of the slice
     float bound;               // no top-k logit is below it
     u64 best;                  // the slice's first ranked token
-    u64 weight[2];             // sums of weights of the slice
+    u64 weight[4];             // sums of weights of the slice: of all, before a cut, of the top k, kept
     unsigned chunk_count[2];   // of this CTA's share of the bins, per level
     u64 chunk_mass[2];
     unsigned listed;           // entries of this CTA's list
     u64 range_hi, range_lo;    // rank order values of the listed bins' tokens
     // Within the CTA.
-    u64 warp_u64[kWarps];
+    u64 warp_u64[kWarps], warp_more[kWarps];
     unsigned warp_u32[kWarps];
     float warp_f32[2][kWarps];
     unsigned digit[256];
@@ -167,7 +167,7 @@ struct Row {
     u64* merged_mass;        // [kHeavyBins / C], then [kSubBins / C]
     int ranks, rank, first;  // CTAs of the cluster, this one, its slice's first token
     int tid, lane, warp;
-    float top, t, per_t, spread, to_bin;
+    float top, t, per_t, spread, to_bin, u;
 
     __device__ Row(const SampleParams& params, Shared& shared) : p(params), sh(shared), cluster(cg::this_cluster()) {}
 
@@ -262,8 +262,8 @@ struct Row {
         __syncthreads();
     }
 
-    // Sum of v over the cluster, for all its threads. `which`: two sums may follow one another
-    // without a barrier between them.
+    // Sum of v over the cluster, for all its threads. `which`: sums that may follow one another
+    // without a barrier of the cluster between them have places of their own.
     __device__ u64 cluster_sum(u64 v, int which) {
         v = warp_sum_u64(v);
         __syncthreads();
@@ -280,8 +280,10 @@ struct Row {
         return all;
     }
 
-    // Sums this CTA's share of the bins over the cluster.
-    __device__ void merge(int level) {
+    // Sums this CTA's share of the bins over the cluster, and the threads' v; returns v's sum.
+    __device__ u64 merge(int level, u64 v) {
+        v = warp_sum_u64(v);
+        if (lane == 0) sh.warp_more[warp] = v;
         cluster.sync();
         const int n = bins_of(level) / ranks, heavy = masses_of(level) / ranks;
         unsigned* counts = merged_count + (level == 0 ? 0 : kBins / ranks);
@@ -309,15 +311,20 @@ struct Row {
         __syncthreads();
         if (tid == 0) {
             unsigned c = 0;
-            u64 m = 0;
+            u64 m = 0, more = 0;
             for (int w = 0; w < kWarps; ++w) {
                 c += sh.warp_u32[w];
                 m += sh.warp_u64[w];
+                more += sh.warp_more[w];
             }
+            sh.weight[0] = more;
             sh.chunk_count[level] = c;
             sh.chunk_mass[level] = m;  // (of level 0 not used: its shares of counts and masses differ)
         }
         cluster.sync();
+        u64 all = 0ull;
+        for (int r = 0; r < ranks; ++r) all += cluster.map_shared_rank(&sh, r)->weight[0];
+        return all;
     }
 
     // Where the running count reaches k (by_mass false) or the running weight `target`.
@@ -546,7 +553,7 @@ struct Row {
                 atomicAdd(raw_count + b, 1u);
                 if (by_mass) atomicAdd(raw_mass + b, weight(x));
             });
-            merge(1);
+            merge(1, 0ull);
             if (!find_bin(1, by_mass, k, target, before_count, before_mass)) return {-INFINITY, 0};
             level = 1;
             const int bin = sh.bin[0];
@@ -559,7 +566,10 @@ struct Row {
             __syncthreads();
         }
         // The remaining tokens, from all CTAs. (At most kOwnList, so that a CTA's list holds them.)
-        if (tid == 0) sh.listed = 0u;
+        if (tid == 0) {
+            sh.listed = 0u;
+            sh.cut = 0ull;
+        }
         __syncthreads();
         each([&](float x, int id) {
             u64 v;
@@ -582,9 +592,8 @@ struct Row {
 
     // The cut among n listed tokens that follow before_count tokens of weight before_mass. The warps
     // of the cluster share the tokens; the lanes of a warp share the others they are ranked against.
+    // (sh.cut was cleared in every CTA before the lists were complete.)
     __device__ Limit ranked_cut(int n, bool by_mass, unsigned k, double target, unsigned before_count, u64 before_mass) {
-        if (tid == 0) sh.cut = 0ull;
-        cluster.sync();
         for (int i = rank * kWarps + warp; i < n; i += ranks * kWarps) {
             const u64 v = list[i];
             unsigned c = 0u;
@@ -616,7 +625,10 @@ struct Row {
         if (sh.bin_count > static_cast<unsigned>(kList)) return false;
         const int bin0 = sh.bin[0], bin1 = sh.bin[1];
         const unsigned before_count = sh.before_count;
-        if (tid == 0) sh.listed = 0u;
+        if (tid == 0) {
+            sh.listed = 0u;
+            sh.cut = 0ull;
+        }
         __syncthreads();
         // Logits above `surely` are in bins before the window, those below `least` behind it (a bin
         // of margin and directed rounding for the edges); between them the bins decide.
@@ -645,7 +657,7 @@ struct Row {
                     if (x[i] >= least && !(x[i] > surely)) {
                         const float d = distance(x[i]);
                         const int bin = d <= spread ? bin_of(d) : kBins;
-                        if (bin >= bin0 && bin <= bin1) append(rank_value(x[i], first + base + lane * V::kN + i), 0ull);
+                            if (bin >= bin0 && bin <= bin1) append(rank_value(x[i], first + base + lane * V::kN + i), weight(x[i]));
                         raised[i] = bin < bin0 ? INFINITY : -INFINITY;
                     }
                 }
@@ -685,10 +697,6 @@ struct Row {
             return false;
         }
         const int own = static_cast<int>(sh.listed);
-        for (int i = tid; i < own; i += kThreads) {
-            own_list[kOwnList + i] = weight(score_from_bits(static_cast<uint32_t>(own_list[i] >> 32)));
-        }
-        cluster.sync();
         limit = ranked_cut(copy_lists(true), true, 0u, target, before_count, before_mass);
         if (limit.x == -INFINITY) return false;  // the cut is not in the window
         // The kept ones of the window, each to the warp that holds it.
@@ -829,24 +837,24 @@ struct Row {
             kept_mass = warp_sum_u64(kept_mass);
             if (lane == 0) {
                 sh.kept = static_cast<int>(kept);
-                sh.weight[0] = kept_mass;
+                sh.weight[3] = kept_mass;
             }
         }
         __syncthreads();
-        const u64 total = sh.weight[0];
-        const u64 target = drawn(row, total);
+        const u64 total = sh.weight[3];
+        const u64 target = drawn(total);
         if (tid < sh.kept) {
             const int id = key_id(ranked[tid]);
             u64 before = 0ull;
-            for (int j = 0; j < sh.kept; ++j) before += key_id(ranked[j]) < id ? ranked[kDirect + j] : 0ull;
+            const int kept = sh.kept;
+#pragma unroll 8
+            for (int j = 0; j < kept; ++j) before += key_id(ranked[j]) < id ? ranked[kDirect + j] : 0ull;
             const u64 w = ranked[kDirect + tid];
             if (target >= before && target < before + w) write(row, id, w, total);
         }
     }
 
-    __device__ __forceinline__ u64 drawn(int row, u64 total) const {
-        float u = p.uniforms[row];
-        u = u >= 0.0f ? fminf(u, 0.99999994f) : 0.0f;
+    __device__ __forceinline__ u64 drawn(u64 total) const {
         const u64 target = static_cast<u64>(floor(static_cast<double>(u) * static_cast<double>(total)));
         return target >= total ? total - 1ull : target;
     }
@@ -867,6 +875,8 @@ __device__ void Row<T>::run() {
     const int share = p.slice / kWarps;
 
     t = p.temperature != nullptr ? p.temperature[row] : 1.0f;
+    u = p.uniforms[row];
+    u = u >= 0.0f ? fminf(u, 0.99999994f) : 0.0f;
     const unsigned k = p.top_k != nullptr && p.top_k[row] > 0 ? static_cast<unsigned>(p.top_k[row]) : 0u;
     const float top_p = p.top_p != nullptr ? p.top_p[row] : 1.0f;
     float min_p = p.min_p != nullptr ? p.min_p[row] : 0.0f;
@@ -1013,15 +1023,15 @@ __device__ void Row<T>::run() {
                 if (by_weight && bin < kHeavyBins) atomicAdd(raw_mass + bin, weight(x));
             });
         }
-        merge(0);
+        u64 total = merge(0, all);
         if (k != 0u) limit = cut(false, k, 0.0);
         if (by_weight) {
             if (k != 0u) {
                 each_from(fmaxf(limit.x, -FLT_MAX), [&](float x, int id) {
                     if (limit.keeps(x, id)) all += weight(x);
                 });
+                total = cluster_sum(all, 2);
             }
-            const u64 total = cluster_sum(all, 0);
             const double target = static_cast<double>(top_p) * static_cast<double>(total);
             // (Below the top-k's total weight, so the cut is not behind the top-k's.)
             summed = cut_and_sum(target, min_p, limit);
@@ -1046,16 +1056,16 @@ __device__ void Row<T>::run() {
     if (tid == 0) {
         u64 all = 0ull;
         for (int w = 0; w < kWarps; ++w) all += sh.warp_u64[w];
-        sh.weight[0] = all;
+        sh.weight[3] = all;
     }
     cluster.sync();
     u64 total = 0ull, before = 0ull;
     for (int r = 0; r < ranks; ++r) {
-        const u64 w = cluster.map_shared_rank(&sh, r)->weight[0];
+        const u64 w = cluster.map_shared_rank(&sh, r)->weight[3];
         if (r < rank) before += w;
         total += w;
     }
-    const u64 target = drawn(row, total);
+    const u64 target = drawn(total);
     for (int w = 0; w < warp; ++w) before += sh.warp_u64[w];
     if (target < before || target >= before + mine) return;
     for (int base = warp * share; base < (warp + 1) * share; base += 32 * V::kN) {
