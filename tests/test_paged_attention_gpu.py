@@ -251,3 +251,28 @@ def test_padding_tokens_are_left_alone(zc):
     out = torch.full_like(q, 9.0)
     zc.paged_attention(cache, batch, q, scale=0.125, out=out)
     assert bool((out[2:] == 9).all()) and bool((out[:2] != 9).all())
+
+
+@pytest.mark.parametrize("page", [3, 8])
+@pytest.mark.parametrize("group,new", [(4, 5), (4, 12), (9, 3), (20, 3), (5, 6)])
+def test_row_tiles_of_32_and_64(zc, group, new, page):
+    """Rows that fill two and four warps, with pages that TMA boxes fit and that they do not."""
+    _run(zc, [new, 1, new - 1], [new + 200, 70, 90], group=group, page=page)
+    _run(zc, [new, 1], [new + 100, 64], group=group, page=page, dim=64, window=40, dtype=torch.float16)
+
+
+@pytest.mark.parametrize("group", [3, 5, 7, 24])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_chunks_of_groups_that_are_no_power_of_two(zc, group, dim):
+    _run(zc, [300, 130], [700, 130], group=group, kv_heads=1, dim=dim)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_chunks_cut_between_many_ctas(zc, dtype):
+    """One unit over far more key tiles than a CTA takes: its parts are joined by a kernel of their own."""
+    _run(zc, [65], [30000], group=1, kv_heads=1, dtype=dtype, page=64)
+    _run(zc, [70, 2], [9000, 5000], group=4, kv_heads=2, dtype=dtype, page=128, window=6000)
+
+
+def test_a_decoding_unit_cut_between_all_ctas(zc):
+    _run(zc, [1], [70001], group=8, kv_heads=1, page=64)

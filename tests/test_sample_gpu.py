@@ -137,3 +137,43 @@ def test_frequencies_follow_the_weights(zc):
     share = torch.bincount(tokens.long(), minlength=5).double() / 4096
     want = torch.softmax(x[0].double(), 0)
     assert bool(((share - want).abs() <= 1 / 4096).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("k", [255, 256, 257, 1000, 5000])
+def test_top_k_around_the_list_that_is_taken_at_once(zc, k, dtype):
+    settings = [(0.9, k, 1.0, 0.0), (1.3, k, 0.97, 0.0), (2.0, k, 0.6, 0.01)]
+    _check(zc, _logits(3, 50000, k, dtype=dtype), settings, [0.2, 0.93, 0.5])
+
+
+@pytest.mark.parametrize("spread", [0.001, 0.3, 30.0, 1000.0])
+def test_flat_and_steep_distributions(zc, spread):
+    settings = [(1.0, 0, 0.9, 0.0), (0.1, 0, 0.5, 0.001), (5.0, 0, 0.999, 0.0), (1.0, 400, 0.9, 0.0)]
+    for dtype in (torch.float32, torch.bfloat16):
+        _check(zc, _logits(4, 30000, 7, spread=spread, dtype=dtype), settings, [0.1, 0.6, 0.99, 0.4])
+
+
+def test_extreme_temperatures(zc):
+    settings = [(1e-30, 0, 0.9, 0.0), (1e-4, 0, 0.9, 0.0), (1e30, 0, 0.3, 0.0), (1e10, 20, 0.5, 0.0), (1e-40, 7, 1.0, 0.0)]
+    _check(zc, _logits(5, 9000, 12), settings, [0.5] * 5)
+
+
+def test_quotients_are_correctly_rounded(zc):
+    """Two tokens at a chosen distance: the drawn token turns at the weight of the correctly rounded quotient, so the
+    logarithm of its probability equals the definition's to the last bit of its fp32 value."""
+    g = torch.Generator().manual_seed(0)
+    rows = 4000
+    distance = torch.rand(rows, generator=g) * 20
+    temperature = (torch.rand(rows, generator=g) + 0.05).float()
+    x = torch.zeros((rows, 2))
+    x[:, 1] = -distance
+    tokens, logprobs = zc.sample(x.cuda(), torch.full((rows,), 0.99999994).cuda(), temperature=temperature.cuda(),
+                                 top_p=torch.full((rows,), 0.99999994).cuda())
+    e = torch.exp((x.cuda()[:, 1] / temperature.cuda()))
+    w = (e.double() * 2.0**40).round()
+    total = w + 2.0**40
+    kept = 2.0**40 < 0.9999999403953552 * total  # whether top-p keeps the second token
+    second = tokens == 1
+    assert bool((second <= kept).all())
+    want = torch.log(torch.where(second, w, torch.full_like(w, 2.0**40)) / torch.where(kept, total, torch.full_like(w, 2.0**40))).float()
+    assert torch.equal(logprobs, want)
