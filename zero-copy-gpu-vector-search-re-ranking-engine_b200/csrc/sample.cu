@@ -262,6 +262,13 @@ struct Row {
         __syncthreads();
     }
 
+    // What CTA `lane` of the cluster shows; lanes past them get `other`. The loads of all CTAs' values
+    // are one (a loop over the CTAs took a remote load's latency for each).
+    template <typename V_, typename F>
+    __device__ __forceinline__ V_ shown(V_ other, F f) const {
+        return lane < ranks ? f(*cluster.map_shared_rank(&sh, lane)) : other;
+    }
+
     // Sum of v over the cluster, for all its threads. `which`: sums that may follow one another
     // without a barrier of the cluster between them have places of their own.
     __device__ u64 cluster_sum(u64 v, int which) {
@@ -275,9 +282,7 @@ struct Row {
             sh.weight[which] = all;
         }
         cluster.sync();
-        u64 all = 0ull;
-        for (int r = 0; r < ranks; ++r) all += cluster.map_shared_rank(&sh, r)->weight[which];
-        return all;
+        return warp_sum_u64(shown(u64{0}, [&](const Shared& o) { return o.weight[which]; }));
     }
 
     // Sums this CTA's share of the bins over the cluster, and the threads' v; returns v's sum.
@@ -322,9 +327,7 @@ struct Row {
             sh.chunk_mass[level] = m;  // (of level 0 not used: its shares of counts and masses differ)
         }
         cluster.sync();
-        u64 all = 0ull;
-        for (int r = 0; r < ranks; ++r) all += cluster.map_shared_rank(&sh, r)->weight[0];
-        return all;
+        return warp_sum_u64(shown(u64{0}, [](const Shared& o) { return o.weight[0]; }));
     }
 
     // Where the running count reaches k (by_mass false) or the running weight `target`.
@@ -336,18 +339,24 @@ struct Row {
     // when no bin reaches it.
     __device__ bool find_bin(int level, bool by_mass, unsigned k, double target, unsigned count, u64 mass) {
         const int n = bins_of(level) / ranks;
-        int owner = -1;
-        for (int r = 0; r < ranks; ++r) {
-            const Shared* other = cluster.map_shared_rank(&sh, r);
-            const unsigned c = other->chunk_count[level];
-            const u64 m = level == 1 ? other->chunk_mass[1] : 0ull;
-            if (reached(by_mass, count + c, mass + m, k, target)) {
-                owner = r;
-                break;
+        // The first CTA whose share of the bins ends at or past the cut.
+        unsigned c_upto = shown(0u, [&](const Shared& o) { return o.chunk_count[level]; });
+        u64 m_upto = level == 1 ? shown(u64{0}, [](const Shared& o) { return o.chunk_mass[1]; }) : 0ull;
+        const unsigned c_share = c_upto;
+        const u64 m_share = m_upto;
+#pragma unroll
+        for (int o = 1; o < kMaxCluster; o <<= 1) {
+            const unsigned tc = __shfl_up_sync(0xffffffffu, c_upto, o);
+            const u64 tm = __shfl_up_sync(0xffffffffu, m_upto, o);
+            if (lane >= o) {
+                c_upto += tc;
+                m_upto += tm;
             }
-            count += c;
-            mass += m;
         }
+        const uint32_t past = __ballot_sync(0xffffffffu, lane < ranks && reached(by_mass, count + c_upto, mass + m_upto, k, target));
+        const int owner = __ffs(past) - 1;
+        count += __shfl_sync(0xffffffffu, c_upto - c_share, owner < 0 ? 0 : owner);
+        mass += __shfl_sync(0xffffffffu, m_upto - m_share, owner < 0 ? 0 : owner);
         if (owner < 0) return false;
         const unsigned* counts = cluster.map_shared_rank(merged_count, owner) + (level == 0 ? 0 : kBins / ranks);
         const u64* masses = cluster.map_shared_rank(merged_mass, owner) + kHeavyBins / ranks;
@@ -686,12 +695,8 @@ struct Row {
         }
         if (per_t != 0.0f && !(min_p > 0.0f)) kept = all;
         const u64 before_mass = cluster_sum(all, 1);
-        unsigned most = 0u, n = 0u;
-        for (int r = 0; r < ranks; ++r) {
-            const unsigned c = cluster.map_shared_rank(&sh, r)->listed;
-            most = max(most, c);
-            n += c;
-        }
+        const unsigned listed = shown(0u, [](const Shared& o) { return o.listed; });
+        const unsigned most = __reduce_max_sync(0xffffffffu, listed), n = __reduce_add_sync(0xffffffffu, listed);
         if (most > static_cast<unsigned>(kOwnList) || n > static_cast<unsigned>(kList)) {
             cluster.sync();  // every CTA has read the counts
             return false;
@@ -724,18 +729,23 @@ struct Row {
 
     // Copies the lists of all CTAs, whose tokens together fit one, into this CTA's; their number.
     __device__ int copy_lists(bool weights) {
-        int n = 0;
-        for (int r = 0; r < ranks; ++r) {
-            const int m = static_cast<int>(cluster.map_shared_rank(&sh, r)->listed);
-            const u64* theirs = cluster.map_shared_rank(own_list, r);
-            for (int i = tid; i < m; i += kThreads) {
-                list[n + i] = theirs[i];
-                if (weights) list[kList + n + i] = theirs[kOwnList + i];
-            }
-            n += m;
+        const int m = static_cast<int>(shown(0u, [](const Shared& o) { return o.listed; }));
+        int upto = m;
+#pragma unroll
+        for (int o = 1; o < kMaxCluster; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+        }
+        // The warps share the CTAs' lists (there are 1, 2, 4 or 8).
+        const int r = warp % ranks, part = warp / ranks;
+        const int count = __shfl_sync(0xffffffffu, m, r), at = __shfl_sync(0xffffffffu, upto - m, r);
+        const u64* theirs = cluster.map_shared_rank(own_list, r);
+        for (int i = part * 32 + lane; i < count; i += kThreads / ranks) {
+            list[at + i] = theirs[i];
+            if (weights) list[kList + at + i] = theirs[kOwnList + i];
         }
         __syncthreads();
-        return n;
+        return __shfl_sync(0xffffffffu, upto, ranks - 1);
     }
 
     // A lower bound of the k-th largest of the threads' values (1 <= k <= kThreads) that shares its
@@ -919,13 +929,8 @@ __device__ void Row<T>::run() {
         }
     }
     cluster.sync();
-    top = -INFINITY;
-    float bound = INFINITY;
-    for (int r = 0; r < ranks; ++r) {
-        const Shared* other = cluster.map_shared_rank(&sh, r);
-        top = fmaxf(top, other->top);
-        bound = fminf(bound, other->bound);
-    }
+    top = warp_max_f32(shown(-INFINITY, [](const Shared& o) { return o.top; }));
+    const float bound = -warp_max_f32(shown(-INFINITY, [](const Shared& o) { return -o.bound; }));
     if (top == -INFINITY) {
         if (rank == 0 && tid == 0) {
             p.tokens[row] = -1;
@@ -943,7 +948,10 @@ __device__ void Row<T>::run() {
         if (lane == 0) atomicMax(&sh.best, best);
         cluster.sync();
         if (rank == 0 && tid == 0) {
-            for (int r = 0; r < ranks; ++r) best = max(best, cluster.map_shared_rank(&sh, r)->best);
+            for (int r = 0; r < ranks; ++r) {
+                const u64 b = cluster.map_shared_rank(&sh, r)->best;
+                best = max(best, b);
+            }
             p.tokens[row] = key_id(best);
             if (p.logprobs != nullptr) p.logprobs[row] = 0.0f;
         }
@@ -956,12 +964,8 @@ __device__ void Row<T>::run() {
     if (direct) {
         each_from(bound, [&](float x, int id) { append(rank_value(x, id), 0ull); });
         cluster.sync();
-        unsigned n = 0u, most = 0u;
-        for (int r = 0; r < ranks; ++r) {
-            const unsigned c = cluster.map_shared_rank(&sh, r)->listed;
-            most = max(most, c);
-            n += c;
-        }
+        const unsigned listed = shown(0u, [](const Shared& o) { return o.listed; });
+        const unsigned most = __reduce_max_sync(0xffffffffu, listed), n = __reduce_add_sync(0xffffffffu, listed);
         if (most <= static_cast<unsigned>(kOwnList) && n <= static_cast<unsigned>(kList)) {
             draw_from_list(row, copy_lists(false), k, top_p, min_p);
             return;
@@ -1059,12 +1063,9 @@ __device__ void Row<T>::run() {
         sh.weight[3] = all;
     }
     cluster.sync();
-    u64 total = 0ull, before = 0ull;
-    for (int r = 0; r < ranks; ++r) {
-        const u64 w = cluster.map_shared_rank(&sh, r)->weight[3];
-        if (r < rank) before += w;
-        total += w;
-    }
+    const u64 weights = shown(u64{0}, [](const Shared& o) { return o.weight[3]; });
+    const u64 total = warp_sum_u64(weights);
+    u64 before = warp_sum_u64(lane < rank ? weights : 0ull);
     const u64 target = drawn(total);
     for (int w = 0; w < warp; ++w) before += sh.warp_u64[w];
     if (target < before || target >= before + mine) return;
