@@ -12,9 +12,9 @@
 // pieces, with the pairs exchanged by shuffles, took 236 instructions per head, and that was the
 // bound: 18,293 tokens of 48 heads in 140 us.)
 //
-// A block takes up to 8 tokens, one after the other: its warps find a token's sequence, position and
-// slot each while the first values are on their way, and every token's values and cosines are
-// loaded while the one before is worked on.
+// A block takes up to 32 tokens, one after the other: its first warp finds their sequences, positions
+// and slots, a token per lane, while the first values are on their way, and every token's values and
+// cosines are loaded while the one before is worked on.
 #include <algorithm>
 
 #include "common.cuh"
@@ -27,7 +27,8 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxHeads = 4;  // of a token, per lane
-constexpr int kMaxTokens = kThreads / 32;  // of a block: a warp finds the place of each
+constexpr int kMaxTokens = 32;  // of a block: a warp finds the places
+constexpr int kBlocksPerSm = 2;
 
 struct AppendParams {
     View view;
@@ -75,7 +76,7 @@ struct Place {
 // HEADS heads of a token per lane, no more than needed. (Two blocks per SM with 128 registers: three
 // with 80 are slower, 123 against 97 us for 18,293 tokens of 48 heads, as the loads ahead spill.)
 template <typename T, int LANES, int HEADS>
-__global__ void __launch_bounds__(kThreads, 2) append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm) append_kernel(const AppendParams p) {
     constexpr int kSegments = kThreads / LANES;
     __shared__ Place s_place[kMaxTokens];
     const View& view = p.view;
@@ -149,10 +150,18 @@ __global__ void __launch_bounds__(kThreads, 2) append_kernel(const AppendParams 
 
     uint2 x[HEADS][2];
     load(x);
-    if (tid / 32 < tokens) {
-        const int token = token0 + tid / 32;
-        const int s = sequence_of(view, token, tid & 31);
-        if ((tid & 31) == 0) {
+    if (tid < 32) {
+        // The first token's sequence, then how many of the next ones begin at or before each token
+        // (32 at a time: there may be empty ones).
+        const int token = token0 + tid;
+        int s = sequence_of(view, token0, tid);
+        for (int next = s + 1;; next += 32) {
+            const int start = next + tid <= view.sequences ? __ldg(view.starts + next + tid) : INT_MAX;
+#pragma unroll 8
+            for (int j = 0; j < 32; ++j) s += __shfl_sync(0xffffffffu, start, j) <= token ? 1 : 0;
+            if (__shfl_sync(0xffffffffu, start, 31) > token0 + tokens - 1) break;
+        }
+        if (tid < tokens) {
             Place place{-1, -2};
             if (s < view.sequences) {
                 const long long end = view.starts[s + 1];
@@ -163,7 +172,7 @@ __global__ void __launch_bounds__(kThreads, 2) append_kernel(const AppendParams 
                 if (p.rotary != nullptr) place.row = turn >= 0 && turn < p.rotary_rows ? static_cast<int>(turn) : -1;
                 if (p.k != nullptr && place.row >= 0) place.slot = slot_offset(view, s, position);
             }
-            s_place[tid / 32] = place;
+            s_place[tid] = place;
         }
     }
     __syncthreads();
@@ -354,9 +363,10 @@ extern "C" int zcgvs_kv_append(const zcgvs_paged_cache* cache, const zcgvs_step_
     p.q_heads = q_heads;
     p.heads = static_cast<int>(heads);
     p.chunks = static_cast<int>(chunks);
-    // Enough blocks to fill the SMs twice over come first, then more tokens per block.
-    const long long fill = 4LL * device_sm_count();
-    p.tokens_per_block = static_cast<int>(std::min<long long>(std::max<long long>(chunks * batch->tokens / fill, 1), kMaxTokens));
+    // As few whole rounds of resident blocks as hold all tokens, evenly filled.
+    const long long resident = static_cast<long long>(kBlocksPerSm) * device_sm_count(), all = chunks * batch->tokens;
+    const long long rounds = (all + resident * kMaxTokens - 1) / (resident * kMaxTokens);
+    p.tokens_per_block = static_cast<int>((all + resident * rounds - 1) / (resident * rounds));
     const unsigned blocks = static_cast<unsigned>(chunks * ((batch->tokens + p.tokens_per_block - 1) / p.tokens_per_block));
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const cudaError_t e = cache->dtype == ZCGVS_DTYPE_F16 ? launch_append_any<__half>(p, blocks, heads_per_lane, s)
