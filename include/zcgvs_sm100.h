@@ -119,7 +119,7 @@ int zcgvs_check_bounded_wait(void* workspace, size_t bytes, void* stream);
  * zcgvs_kernel_timing_read synchronises the recorded events of `tag` and returns their summed
  * duration and count. Tags: "scan" (streaming scan), "gemm_sample", "gemm_threshold",
  * "gemm_filter", "gemm_bucket", "gemm_select", "gemm_retry", "gemm_emit", "rescore", "lexical",
- * "merge". */
+ * "merge"; "kv_append", "paged_stream", "paged_chunk", "paged_join", "sample" (the answer step). */
 int zcgvs_kernel_timing(int enable);
 int zcgvs_kernel_timing_read(const char* tag, double* total_ms, int* launches);
 
